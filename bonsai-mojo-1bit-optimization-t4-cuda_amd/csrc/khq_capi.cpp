@@ -991,6 +991,8 @@ int khq_attn_step_batched_fp16(const khq_seq* seqs, int n_seq, const void* centr
 
 namespace khq {
 
+hipError_t shared_workspace(size_t bytes, hipStream_t stream, float** out);
+
 bool step_window_in_ws(int H_q, int H_kv, int c_len, int win_len) {
     return H_kv > 0 && H_q % H_kv == 0 && c_len > 0 && win_len > 0 && win_len <= 256 &&
            g_kernel_choice.load(std::memory_order_relaxed) == 0 && use_mfma(H_q / H_kv, H_kv, 1);
@@ -1001,6 +1003,11 @@ int attn_step_append(const AttnArgs& a, int H_q, __half* out, hipStream_t stream
                           a.cents_k, a.cents_v, a.vq, a.rotor_k, a.rotor_v, a.dk, a.dv, a.ring_k,
                           a.ring_v, out, H_q, a.h_kv, a.c_len, a.win_start, a.win_len, a.ring_cap,
                           a.sc, a.a_k, a.a_v, a.rope_base, stream, false, &a.add);
+}
+
+// The workspace for launchers outside this library (khq_paged_internal.h).
+hipError_t shared_workspace(size_t bytes, hipStream_t stream, float** out) {
+    return workspace(bytes, stream, out);
 }
 
 int prefill_attn_run(PrefillArgs a, const RingArgs* ring, hipStream_t stream, bool merge) {

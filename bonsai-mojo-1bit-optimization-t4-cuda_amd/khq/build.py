@@ -1,4 +1,5 @@
-"""Compiles the HIP library khq/libkhq_hip.so for gfx950 with hipcc."""
+"""Compiles the HIP libraries khq/libkhq_hip.so and khq/libkhq_paged.so (the
+paged cache, linked to the first) for gfx950 with hipcc."""
 from __future__ import annotations
 
 import os
@@ -14,6 +15,9 @@ LIB_NAME = "libkhq_hip.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["khq_kernels.hip", "khq_attn_ws.hip", "khq_finish.hip", "khq_prefill.hip", "khq_dump.hip", "khq_calib.hip",
            "khq_capi.cpp", "khq_layer.cpp"]
+PAGED_LIB_NAME = "libkhq_paged.so"
+PAGED_LIB_PATH = os.path.join(PKG_DIR, PAGED_LIB_NAME)
+PAGED_SOURCES = ["khq_paged.hip", "khq_paged_attn.hip", "khq_paged_capi.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("KHQ_OFFLOAD_ARCH", "gfx950")
@@ -27,16 +31,22 @@ FLAGS = [
 ]
 
 
-def build(verbose: bool = False) -> str:
+def _compile(sources, path: str, extra, verbose: bool) -> None:
     cmd = [HIPCC, *FLAGS, "-I", INCLUDE, "-I", CSRC,
-           *[os.path.join(CSRC, s) for s in SOURCES], "-o", LIB_PATH + ".tmp"]
+           *[os.path.join(CSRC, s) for s in sources], *extra, "-o", path + ".tmp"]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError(f"hipcc failed ({res.returncode}) building {LIB_NAME}")
-    os.replace(LIB_PATH + ".tmp", LIB_PATH)
+        raise RuntimeError(f"hipcc failed ({res.returncode}) building {os.path.basename(path)}")
+    os.replace(path + ".tmp", path)
+
+
+def build(verbose: bool = False) -> str:
+    _compile(SOURCES, LIB_PATH, [], verbose)
+    _compile(PAGED_SOURCES, PAGED_LIB_PATH,
+             ["-L", PKG_DIR, f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN"], verbose)
     return LIB_PATH
 
 
