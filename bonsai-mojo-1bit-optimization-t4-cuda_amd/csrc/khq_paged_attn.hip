@@ -1,14 +1,526 @@
 // khq_paged_attn.hip -- attention of new tokens over a paged cache.
+//
+// The rows of one KV head of a sequence, row r = query token r / n_rep, head
+// r % n_rep of its group, are cut into row tiles, and where those are fewer
+// than the chip's blocks, a tile's keys into splits whose partial results
+// (unnormalised sum, maximum, sum of weights) a second launch joins in order.
+// Everything about lengths is read on the device, so a captured launch follows
+// them: each wavefront derives the whole partition from cu_q and seq_kv again
+// (schedule below), which for one sequence is a few scalar operations and for
+// some hundred one pass of a wavefront, about a microsecond.
+//
+// Two kernels share the sequences by their row count: up to 16 rows (a decode
+// step's 6 of 24 / 4 heads) stream keys and values through registers
+// (attn_stream_kernel), more go in tiles of 128 or 256 rows that share keys
+// and values in LDS (attn_tile_kernel).
 #include "khq_paged_internal.h"
+
+#include <algorithm>
 
 namespace khq {
 namespace paged {
 namespace {
 
-// One wavefront a (row, head): the keys one after the other, running maximum
-// and sum.
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+// the caller's rows: any address of a 16-bit element
+typedef uint32_t u4e __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u2e __attribute__((ext_vector_type(2), aligned(2)));
+
+template <typename T>
+struct V {
+    typedef T x2 __attribute__((ext_vector_type(2)));
+    typedef T x4 __attribute__((ext_vector_type(4)));
+    typedef T x8 __attribute__((ext_vector_type(8)));
+};
+__device__ __forceinline__ f4 mfma16(V<fp16>::x8 a, V<fp16>::x8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f4 mfma16(V<bf16>::x8 a, V<bf16>::x8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16v mfma32(V<fp16>::x8 a, V<fp16>::x8 b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16v mfma32(V<bf16>::x8 a, V<bf16>::x8 b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+// Two floats rounded to the type (to nearest even).
+template <typename T>
+__device__ __forceinline__ uint32_t pack(float x, float y) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x, y}, typename V<T>::x2));
+}
+// l plus the two values of a packed pair.
+template <typename T>
+__device__ __forceinline__ float add_pair(uint32_t p, float l) {
+    typedef typename V<T>::x2 x2;
+    const x2 v = __builtin_bit_cast(x2, p);
+    if constexpr (__is_same(T, fp16)) {
+        return __builtin_amdgcn_fdot2(v, x2{(T)1.0f, (T)1.0f}, l, false);
+    } else {
+        return l + ((float)v[0] + (float)v[1]);
+    }
+}
+// Whether either 16-bit value of a pair is an infinity or a NaN.
+template <typename T>
+__device__ __forceinline__ bool nonfinite_pair(uint32_t p) {
+    const uint32_t e = __is_same(T, fp16) ? 0x7c00u : 0x7f80u;
+    return (p & e) == e || (p & (e << 16)) == (e << 16);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t finite_pair(uint32_t p) {  // those as zeros
+    const uint32_t e = __is_same(T, fp16) ? 0x7c00u : 0x7f80u;
+    if ((p & e) == e) p &= 0xffff0000u;
+    if ((p & (e << 16)) == (e << 16)) p &= 0xffffu;
+    return p;
+}
+template <typename T>
+__device__ __forceinline__ float sigmoid(T g) {
+    return 1.0f / (1.0f + __expf(-(float)g));
+}
+
+// Reference maximum of a row that has seen no key: finite, so that a masked
+// score (-inf) less it is -inf and its weight 0 without a test.
+constexpr float M_NONE = -1e30f;
+constexpr float LOG2E = 1.44269504f;
+// A row's reference rises only when a score passes it by this (in log2 units):
+// weights stay below e^10, far from the type's largest value.
+constexpr float GAP = 10.0f * LOG2E;
+
+// Scores in log2 units, so that a weight is one exp2; not 0, whose product
+// with a masked score would be no number.
+__device__ __forceinline__ float score_scale(float scale) {
+    return fmaxf(fabsf(scale) * LOG2E, 1e-30f);
+}
+
+// ------------------------------------------------------------ the partition
+constexpr int SMALL_ROWS = 16;
+constexpr int STREAM_WAVES = 4;
+constexpr int STREAM_UNIT = 32 * STREAM_WAVES;  // keys: a 32-key tile for each wavefront
+constexpr int STREAM_SLOTS = 512;               // blocks that run at once, two a CU
+constexpr int TILE_UNIT = 64;
+constexpr int TILE_SLOTS = 256;
+
+// Which sequences a launch serves: by their rows, or all of them.
+enum Serve { SERVE_SMALL, SERVE_LARGE, SERVE_ALL };
+
+struct Part {
+    int rows;   // of a row tile
+    int unit;   // keys
+    int slots;  // blocks
+    Serve serve;
+    bool split;  // whether keys may be split
+};
+
+struct Item {
+    int seq, row0, n_q, kv;  // sequence, its first batch row, rows and tokens
+    int head, qt, split, n_split;
+    int block;  // of split 0; split i is block + i * H_kv
+};
+
+struct SeqLen {
+    int row0, n_q, kv, tiles, units;  // tiles: row tiles (0: not served)
+};
+
+__device__ __forceinline__ SeqLen seq_len(const AttnArgs& a, const Part& pt, int s) {
+    SeqLen l;
+    const int c0 = min(max(a.r.cu_q[s], 0), a.r.n_tok), c1 = min(max(a.r.cu_q[s + 1], 0), a.r.n_tok);
+    l.row0 = c0;
+    l.n_q = max(c1 - c0, 0);
+    l.kv = min(max(a.r.seq_kv[s], 0), a.r.table_ld * a.p.page_size);
+    const int rows = l.n_q * a.n_rep;
+    const bool mine = pt.serve == SERVE_ALL || (rows <= SMALL_ROWS) == (pt.serve == SERVE_SMALL);
+    l.tiles = mine ? (rows + pt.rows - 1) / pt.rows : 0;
+    // units of the middle row: what a tile costs on average
+    l.units = max(1, (max(l.kv - l.n_q / 2, 0) + pt.unit - 1) / pt.unit);
+    return l;
+}
+
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// Item x of the launch (joining: of those that are split).  Items are numbered
+// sequence by sequence; within one, KV heads in turn (blocks go to the XCDs in
+// turn, so a head's row tiles meet its keys in one L2), then splits, then row
+// tiles from the last, which sees most keys, to the first.  With items fewer
+// than slots the keys are split by the unit count u = cost / (slots - items):
+// sum of ceil(units / u) <= cost / u + items <= slots.
+__device__ __forceinline__ bool schedule(const AttnArgs& a, const Part& pt, int x, bool joining,
+                                         Item& it) {
+    const int lane = threadIdx.x & 63, n_seq = a.r.n_seq, h_kv = a.p.H_kv;
+    const int per = (n_seq + 63) >> 6, s0 = lane * per, s1 = min(s0 + per, n_seq);
+    SeqLen one{};
+    int items = 0;
+    long long cost = 0;
+    for (int s = s0; s < s1; s++) {
+        one = seq_len(a, pt, s);
+        items += one.tiles * h_kv;
+        cost += (long long)one.tiles * h_kv * one.units;
+    }
+    int u = 0x7fffffff;
+    if (pt.split) {
+        const int all = wave_sum(items);
+        if (all < pt.slots) {
+            const int room = pt.slots - all;
+            u = (int)min((wave_sum(cost) + room - 1) / room, 0x7fffffffll);
+            u = max(u, 1);
+        }
+    }
+    auto splits = [&](const SeqLen& l) { return (int)(((long long)l.units + u - 1) / u); };
+    int blocks = 0, found = 0;  // of this lane's sequences
+    for (int s = s0; s < s1; s++) {
+        if (per > 1) one = seq_len(a, pt, s);
+        const int n = one.tiles * h_kv, sp = splits(one);
+        blocks += n * sp;
+        found += joining ? (sp > 1 ? n : 0) : n * sp;
+    }
+    int upto = found, upto_b = blocks;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(upto, o, 64), z = __shfl_up(upto_b, o, 64);
+        if (lane >= o) {
+            upto += y;
+            upto_b += z;
+        }
+    }
+    const unsigned long long past = __ballot(upto > x);
+    if (past == 0) return false;
+    const int owner = __ffsll(past) - 1;
+    // the owner walks its sequences
+    int at = upto - found, block = upto_b - blocks, seq = s0;
+    if (lane == owner) {
+        for (int s = s0; s < s1; s++) {
+            if (per > 1) one = seq_len(a, pt, s);
+            seq = s;
+            const int n = one.tiles * h_kv, sp = splits(one);
+            const int c = joining ? (sp > 1 ? n : 0) : n * sp;
+            if (x < at + c) break;
+            at += c;
+            block += n * sp;
+        }
+    }
+    auto from = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
+    it.seq = from(seq);
+    it.row0 = from(one.row0);
+    it.n_q = from(one.n_q);
+    it.kv = from(one.kv);
+    it.n_split = from(splits(one));
+    const int tiles = from(one.tiles), j = x - from(at);
+    it.block = from(block);
+    it.head = j % h_kv;
+    const int k = j / h_kv;
+    it.split = joining ? 0 : k % it.n_split;
+    const int q = joining ? k : k / it.n_split;  // row tiles from the last
+    it.qt = tiles - 1 - q;
+    it.block += q * it.n_split * h_kv + it.head;
+    return true;
+}
+
+// Tokens that row r of the item's sequence sees.
+__device__ __forceinline__ int visible(const AttnArgs& a, const Item& it, int r) {
+    return min(it.kv, max(0, it.kv - it.n_q + a.by_rep.div(r) + 1));
+}
+// Element offset of token t of a sequence in the pages (0 and bad set for a
+// table entry outside the cache).
+__device__ __forceinline__ long long token_at(const AttnArgs& a, const Item& it, int t, bool& bad) {
+    const int pg = a.by_page.div(t), in = t - pg * a.p.page_size;
+    int e = a.r.table[(size_t)it.seq * a.r.table_ld + pg];
+    bad = (unsigned)e >= (unsigned)a.p.n_pages;
+    e = bad ? 0 : e;
+    return e * a.p.page_stride + in * a.p.token_stride + it.head * a.p.head_stride;
+}
+
+// Partial results: f32 [block][rows][D] (each kernel's own order of a block's
+// values), then (maximum, sum) f32 pairs [block][rows].
+__device__ __forceinline__ float* part_acc(float* ws, const Part& pt, int d, int block) {
+    return ws + (size_t)block * pt.rows * d;
+}
+__device__ __forceinline__ float2* part_ml(float* ws, const Part& pt, int d, int block) {
+    return reinterpret_cast<float2*>(ws + (size_t)pt.slots * pt.rows * d) + (size_t)block * pt.rows;
+}
+
+// ------------------------------------------------------------ few rows
+// A wavefront takes 32-key tiles by itself, 16 rows on 16x16x32 MFMAs.  MFMA
+// operands come straight from global loads: S^T = K Q^T takes K rows as they
+// lie (lane: key, 8 dims); its result (row = lane % 16, keys 4 (lane / 16) + r
+// of both 16-key halves) is the B operand of O^T += V^T P^T when that
+// product's K index 8 g + j stands for key 4 g + j (j < 4) and 16 + 4 g + j - 4;
+// a lane loads those 8 keys' values of 8 consecutive dims and transposes them
+// in its registers (32 byte permutes), dim 8 m + t standing for row m of
+// product t.  No LDS and no barrier until the block's wavefronts join.
 template <typename T, int D>
-__global__ __launch_bounds__(64) void attn_row_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnArgs a, Part pt) {
+    constexpr int NW = STREAM_WAVES, KS = D / 32;          // K steps of a score
+    constexpr int VE = D == 64 ? 4 : 8, NH = D / 16 / VE;  // dims a lane loads at once, times
+    constexpr int LD = D + 4;
+    typedef typename V<T>::x8 x8;
+    __shared__ union __align__(16) {
+        T q[16][D + 8];
+        float acc[NW][16][LD];
+    } lds;
+    __shared__ float s_m[NW][16], s_l[NW][16];
+    Item it;
+    if (!schedule(a, pt, blockIdx.x, false, it)) return;
+    const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+    const int rows = min(16, it.n_q * a.n_rep - it.qt * 16);  // of this tile
+    const int r0 = it.qt * 16;
+    // ---- queries into LDS, the scale's sign with them
+    const uint32_t flip = a.r.scale < 0.0f ? 0x80008000u : 0u;
+    for (int i = tid; i < 16 * (D / 8); i += 64 * NW) {
+        const int row = i / (D / 8), c = i % (D / 8);
+        u4e v = {0u, 0u, 0u, 0u};
+        if (row < rows) {
+            const int r = r0 + row, tok = a.by_rep.div(r), hq = it.head * a.n_rep + r - tok * a.n_rep;
+            v = *reinterpret_cast<const u4e*>((const T*)a.r.q + (it.row0 + tok) * a.r.q_token +
+                                              hq * a.r.q_head + 8 * c);
+        }
+        *reinterpret_cast<u4*>(&lds.q[row][8 * c]) = u4{v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip};
+    }
+    __syncthreads();
+    x8 qf[KS];
+#pragma unroll
+    for (int st = 0; st < KS; st++) qf[st] = *reinterpret_cast<const x8*>(&lds.q[li][32 * st + 8 * lg]);
+    const int vis = li < rows ? visible(a, it, r0 + li) : 0;
+    const int vis_lo = visible(a, it, r0), vis_hi = visible(a, it, r0 + rows - 1);
+    const int units = (vis_hi + STREAM_UNIT - 1) / STREAM_UNIT;
+    const int t_lo = (int)((long long)units * it.split / it.n_split) * NW;
+    const int t_hi = min((int)((long long)units * (it.split + 1) / it.n_split) * NW, (vis_hi + 31) >> 5);
+    const float sc2 = score_scale(a.r.scale);
+    const T* kp = (const T*)a.p.k;
+    const T* vp = (const T*)a.p.v;
+    f4 acc[NH][VE];
+#pragma unroll
+    for (int h = 0; h < NH; h++)
+#pragma unroll
+        for (int t = 0; t < VE; t++) acc[h][t] = f4{0.f, 0.f, 0.f, 0.f};
+    float m_ref = M_NONE, l_part = 0.0f;
+    for (int t = t_lo + wv; t < t_hi; t += NW) {
+        const int key0 = t * 32;
+        // a lane's key: tokens past the last one seen stand for it
+        bool bad;
+        const long long off = token_at(a, it, min(key0 + (lane & 31), vis_hi - 1), bad);
+        const unsigned long long bad_keys = __ballot(bad);
+        u4 kr[2][KS];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const T* src = kp + __shfl(off, 16 * h + li, 64) + 8 * lg;
+#pragma unroll
+            for (int st = 0; st < KS; st++) kr[h][st] = *reinterpret_cast<const u4*>(src + 32 * st);
+        }
+        uint32_t vr[8][NH][VE / 2];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const T* src = vp + __shfl(off, (j & 4) * 4 + 4 * lg + (j & 3), 64) + VE * li;
+#pragma unroll
+            for (int h = 0; h < NH; h++) {
+                if constexpr (VE == 8) {
+                    const u4 v = *reinterpret_cast<const u4*>(src + 128 * h);
+                    vr[j][h][0] = v.x; vr[j][h][1] = v.y; vr[j][h][2] = v.z; vr[j][h][3] = v.w;
+                } else {
+                    const u2 v = *reinterpret_cast<const u2*>(src);
+                    vr[j][h][0] = v.x; vr[j][h][1] = v.y;
+                }
+            }
+        }
+        f4 s[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            s[h] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < KS; st++) s[h] = mfma16(__builtin_bit_cast(x8, kr[h][st]), qf[st], s[h]);
+        }
+        // ---- mask: keys 16 h + 4 lg + r of row li
+        float sc[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) sc[e] = s[e >> 2][e & 3];
+        if (bad_keys) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (bad_keys >> (16 * (e >> 2) + 4 * lg + (e & 3)) & 1) sc[e] = __builtin_nanf("");
+        }
+        if (key0 + 32 > vis_lo || rows < 16) {  // (rows past the tile's see nothing)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (key0 + 16 * (e >> 2) + 4 * lg + (e & 3) >= vis) sc[e] = -INFINITY;
+        }
+        bool odd = false;  // values that are no numbers where a row's mask has to hold
+        if (key0 + 32 > vis_lo) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const bool none = key0 + (j & 4) * 4 + 4 * lg + (j & 3) >= vis_hi;
+#pragma unroll
+                for (int h = 0; h < NH; h++)
+#pragma unroll
+                    for (int w = 0; w < VE / 2; w++) {
+                        if (none) vr[j][h][w] = 0u;
+                        odd = odd || nonfinite_pair<T>(vr[j][h][w]);
+                    }
+            }
+            odd = __ballot(odd) != 0ull;
+        }
+        // ---- running maximum, raised only when it must be
+        float lmax = sc[0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) lmax = fmaxf(lmax, sc[e]);
+        lmax *= sc2;
+        if (__ballot(lmax > m_ref + GAP) != 0ull) {
+            lmax = fmaxf(lmax, __shfl_xor(lmax, 16, 64));
+            lmax = fmaxf(lmax, __shfl_xor(lmax, 32, 64));
+            const float m_new = fmaxf(m_ref, lmax);
+            const float fac = __builtin_amdgcn_exp2f(m_ref - m_new);  // 0 from M_NONE, 1 where it stays
+            m_ref = m_new;
+            l_part *= fac;
+#pragma unroll
+            for (int h = 0; h < NH; h++)
+#pragma unroll
+                for (int e = 0; e < VE; e++) acc[h][e] *= fac;
+        }
+        uint32_t pw[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            pw[e] = pack<T>(__builtin_amdgcn_exp2f(fmaf(sc[2 * e], sc2, -m_ref)),
+                            __builtin_amdgcn_exp2f(fmaf(sc[2 * e + 1], sc2, -m_ref)));
+            l_part = add_pair<T>(pw[e], l_part);
+        }
+        const x8 pb = __builtin_bit_cast(x8, u4{pw[0], pw[1], pw[2], pw[3]});
+        if (odd) {
+            // 0 * inf is no 0: such values leave the product and join the rows that see them
+            for (int k = 0; k < 32; k++) {
+                const T* src = vp + __shfl(off, k, 64);
+                const bool sees = key0 + k < vis;
+#pragma unroll
+                for (int h = 0; h < NH; h++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+#pragma unroll
+                        for (int e = 0; e < VE; e++) {
+                            const float v = (float)src[VE * 16 * h + VE * (4 * lg + r) + e];
+                            acc[h][e][r] += sees && !(fabsf(v) < INFINITY) ? v : 0.0f;
+                        }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int h = 0; h < NH; h++)
+#pragma unroll
+                    for (int w = 0; w < VE / 2; w++) vr[j][h][w] = finite_pair<T>(vr[j][h][w]);
+        }
+#pragma unroll
+        for (int h = 0; h < NH; h++)
+#pragma unroll
+            for (int e = 0; e < VE; e++) {
+                uint32_t w[4];
+                const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    w[i] = __builtin_amdgcn_perm(vr[2 * i + 1][h][e >> 1], vr[2 * i][h][e >> 1], sel);
+                acc[h][e] = mfma16(__builtin_bit_cast(x8, u4{w[0], w[1], w[2], w[3]}), pb, acc[h][e]);
+            }
+    }
+    // ---- the wavefronts join in LDS
+    l_part += __shfl_xor(l_part, 16, 64);
+    l_part += __shfl_xor(l_part, 32, 64);
+    __syncthreads();  // queries read
+    if (lg == 0) {
+        s_m[wv][li] = m_ref;
+        s_l[wv][li] = l_part;
+    }
+#pragma unroll
+    for (int h = 0; h < NH; h++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int e = 0; e < VE; e += 4)
+                *reinterpret_cast<f4*>(&lds.acc[wv][li][VE * 16 * h + VE * (4 * lg + r) + e]) =
+                    f4{acc[h][e][r], acc[h][e + 1][r], acc[h][e + 2][r], acc[h][e + 3][r]};
+    __syncthreads();
+    float* ws = static_cast<float*>(a.r.ws);
+    const bool direct = it.n_split == 1;
+    const int block = it.block + it.split * a.p.H_kv;
+    for (int i = tid; i < rows * (D / 4); i += 64 * NW) {
+        const int row = i / (D / 4), c = (i % (D / 4)) * 4;
+        float m = s_m[0][row];
+#pragma unroll
+        for (int w = 1; w < NW; w++) m = fmaxf(m, s_m[w][row]);
+        f4 o = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float f = __builtin_amdgcn_exp2f(s_m[w][row] - m);
+            o += *reinterpret_cast<const f4*>(&lds.acc[w][row][c]) * f;
+            l += s_l[w][row] * f;
+        }
+        if (direct) {
+            const int r = r0 + row, tok = a.by_rep.div(r), hq = it.head * a.n_rep + r - tok * a.n_rep;
+            const float inv = visible(a, it, r) > 0 ? 1.0f / l : 0.0f;
+            o *= inv;
+            if (a.r.gate) {
+                const u2e g = *reinterpret_cast<const u2e*>(
+                    (const T*)a.r.gate + (it.row0 + tok) * a.r.gate_token + hq * a.r.gate_head + c);
+                const typename V<T>::x4 gv = __builtin_bit_cast(typename V<T>::x4, u2{g.x, g.y});
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] *= sigmoid(gv[e]);
+            }
+            *reinterpret_cast<u2e*>((T*)a.r.out + (it.row0 + tok) * a.r.out_token + hq * a.r.out_head + c) =
+                u2e{pack<T>(o[0], o[1]), pack<T>(o[2], o[3])};
+        } else {
+            *reinterpret_cast<f4*>(part_acc(ws, pt, D, block) + row * D + c) = o;
+            if (c == 0) part_ml(ws, pt, D, block)[row] = float2{m, l};
+        }
+    }
+}
+
+// The splits of one row: each wavefront sums every fourth, the four meet in LDS.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_stream_join_kernel(AttnArgs a, Part pt) {
+    constexpr int E = D / 64;
+    __shared__ float s_o[4][D], s_l[4];
+    Item it;
+    if (!schedule(a, pt, blockIdx.x >> 4, true, it)) return;
+    const int row = blockIdx.x & 15, r = it.qt * 16 + row;
+    if (r >= it.n_q * a.n_rep) return;
+    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, h_kv = a.p.H_kv;
+    float* ws = static_cast<float*>(a.r.ws);
+    float m = M_NONE;
+    for (int i = lane; i < it.n_split; i += 64)
+        m = fmaxf(m, part_ml(ws, pt, D, it.block + i * h_kv)[row].x);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    float o[E] = {}, l = 0.0f;
+#pragma unroll 4
+    for (int i = wv; i < it.n_split; i += 4) {
+        const float2 ml = part_ml(ws, pt, D, it.block + i * h_kv)[row];
+        const float* acc = part_acc(ws, pt, D, it.block + i * h_kv) + row * D + E * lane;
+        const float f = __builtin_amdgcn_exp2f(ml.x - m);
+        l += ml.y * f;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] += acc[e] * f;
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) s_o[wv][E * lane + e] = o[e];
+    if (lane == 0) s_l[wv] = l;
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c >= D) return;
+    float v = (s_o[0][c] + s_o[1][c]) + (s_o[2][c] + s_o[3][c]);
+    l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    const int tok = a.by_rep.div(r), hq = it.head * a.n_rep + r - tok * a.n_rep;
+    v *= visible(a, it, r) > 0 ? 1.0f / l : 0.0f;
+    if (a.r.gate)
+        v *= sigmoid(((const T*)a.r.gate)[(it.row0 + tok) * a.r.gate_token + hq * a.r.gate_head + c]);
+    ((T*)a.r.out)[(it.row0 + tok) * a.r.out_token + hq * a.r.out_head + c] = (T)v;
+}
+
+// One wavefront a (row, head): the keys one after the other.
+template <typename T, int D>
+__global__ __launch_bounds__(64) void attn_row_kernel(AttnArgs a, Part pt) {
     const khq_attn_rows& r = a.r;
     const int row = blockIdx.x, hq = blockIdx.y, lane = threadIdx.x;
     int lo = 0, hi = r.n_seq;  // the last sequence whose first row is not past row
@@ -19,6 +531,7 @@ __global__ __launch_bounds__(64) void attn_row_kernel(AttnArgs a) {
     }
     const int first = r.cu_q[lo], end = r.cu_q[lo + 1];
     if (row < first || row >= end) return;
+    if (pt.serve == SERVE_LARGE && (end - first) * a.n_rep <= SMALL_ROWS) return;
     const long long cap = (long long)r.table_ld * a.p.page_size;
     const int kv = (int)min((long long)max(r.seq_kv[lo], 0), cap);
     const int vis = min(kv, kv - (end - first) + (row - first) + 1);
@@ -54,23 +567,57 @@ __global__ __launch_bounds__(64) void attn_row_kernel(AttnArgs a) {
     }
 }
 
-}  // namespace
+// What a call of these sizes launches.
+struct Plan {
+    bool stream, tile;
+    Part ps, pl;
+    int stream_blocks;
+};
+Plan plan_of(int n_tok, int n_seq, int H_q, int H_kv, int max_q) {
+    const int n_rep = H_q / H_kv;
+    Plan p{};
+    p.stream = true;  // there may be short sequences whatever max_q says
+    p.tile = (long long)max_q * n_rep > SMALL_ROWS;
+    p.ps = Part{16, STREAM_UNIT, STREAM_SLOTS, p.tile ? SERVE_SMALL : SERVE_ALL, true};
+    p.pl = Part{0, 0, 0, SERVE_LARGE, false};
+    // row tiles there may be: those served hold 16 rows or, served all, n_tok's
+    const long long most = p.tile ? (long long)std::min(n_tok, n_seq) * H_kv
+                                  : ((long long)n_tok * n_rep / 16 + std::min(n_tok, n_seq)) * H_kv;
+    p.stream_blocks = (int)std::max<long long>(STREAM_SLOTS, most);
+    return p;
+}
+size_t part_bytes(const Part& pt, int d) {
+    return (size_t)pt.slots * pt.rows * (d * sizeof(float) + sizeof(float2));
+}
 
-size_t attn_ws_bytes(int, int, int, int, int, int) { return 0; }
-
-template <typename T>
-static hipError_t attn_of(const AttnArgs& a, hipStream_t st) {
-    const dim3 grid(a.r.n_tok, a.r.H_q);
-    switch (a.p.head_dim) {
-        case 64: hipLaunchKernelGGL((attn_row_kernel<T, 64>), grid, dim3(64), 0, st, a); break;
-        case 128: hipLaunchKernelGGL((attn_row_kernel<T, 128>), grid, dim3(64), 0, st, a); break;
-        default: hipLaunchKernelGGL((attn_row_kernel<T, 256>), grid, dim3(64), 0, st, a); break;
+template <typename T, int D>
+hipError_t launch(const AttnArgs& a, hipStream_t st) {
+    const Plan p = plan_of(a.r.n_tok, a.r.n_seq, a.r.H_q, a.p.H_kv, a.r.max_q);
+    if (p.tile)
+        hipLaunchKernelGGL((attn_row_kernel<T, D>), dim3(a.r.n_tok, a.r.H_q), dim3(64), 0, st, a, p.pl);
+    if (p.stream) {
+        hipLaunchKernelGGL((attn_stream_kernel<T, D>), dim3(p.stream_blocks), dim3(64 * STREAM_WAVES), 0,
+                           st, a, p.ps);
+        hipLaunchKernelGGL((attn_stream_join_kernel<T, D>), dim3(STREAM_SLOTS * 16), dim3(256), 0, st, a,
+                           p.ps);
     }
     return hipGetLastError();
 }
 
+}  // namespace
+
+size_t attn_ws_bytes(int n_tok, int n_seq, int H_q, int H_kv, int head_dim, int max_q) {
+    const Plan p = plan_of(n_tok, n_seq, H_q, H_kv, max_q);
+    return std::max(part_bytes(p.ps, head_dim), part_bytes(p.pl, head_dim));
+}
+
 hipError_t launch_attn(const AttnArgs& a, hipStream_t st) {
-    return a.p.dtype == KHQ_FP16 ? attn_of<fp16>(a, st) : attn_of<bf16>(a, st);
+    const bool half = a.p.dtype == KHQ_FP16;
+    switch (a.p.head_dim) {
+        case 64: return half ? launch<fp16, 64>(a, st) : launch<bf16, 64>(a, st);
+        case 128: return half ? launch<fp16, 128>(a, st) : launch<bf16, 128>(a, st);
+        default: return half ? launch<fp16, 256>(a, st) : launch<bf16, 256>(a, st);
+    }
 }
 
 }  // namespace paged

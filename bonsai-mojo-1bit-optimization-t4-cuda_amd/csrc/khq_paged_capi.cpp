@@ -79,7 +79,7 @@ int khq_qk_norm_rope(const khq_rows* rows, const khq_pages* pages, hipStream_t s
 
 static bool attn_sizes_ok(int n_tok, int n_seq, int H_q, int H_kv, int head_dim, int max_q) {
     return n_tok >= 0 && n_seq > 0 && n_seq <= KHQ_PAGED_MAX_SEQ && H_q > 0 && H_kv > 0 &&
-           H_q % H_kv == 0 && dim_ok(head_dim) && max_q > 0;
+           H_q % H_kv == 0 && dim_ok(head_dim) && max_q > 0 && (long long)n_tok * H_q < 0x7fffffffLL;
 }
 
 long long khq_paged_attn_ws_bytes(int n_tok, int n_seq, int H_q, int H_kv, int head_dim, int max_q) {
@@ -99,6 +99,8 @@ int khq_paged_attn(const khq_attn_rows* rows, const khq_pages* pages, hipStream_
     a.r = r;
     a.p = *pages;
     a.n_rep = r.H_q / pages->H_kv;
+    a.by_page = khq::FastDiv(pages->page_size);
+    a.by_rep = khq::FastDiv(a.n_rep);
     const size_t need = khq::paged::attn_ws_bytes(r.n_tok, r.n_seq, r.H_q, pages->H_kv,
                                                   pages->head_dim, r.max_q);
     if (r.ws) {

@@ -38,9 +38,10 @@ struct RowsArgs {
 hipError_t launch_rows(const RowsArgs& a, hipStream_t st);
 
 struct AttnArgs {
-    khq_attn_rows r;
+    khq_attn_rows r;  // ws set
     khq_pages p;
     int n_rep;
+    FastDiv by_page, by_rep;  // page_size, n_rep
 };
 hipError_t launch_attn(const AttnArgs& a, hipStream_t st);
 size_t attn_ws_bytes(int n_tok, int n_seq, int H_q, int H_kv, int head_dim, int max_q);
