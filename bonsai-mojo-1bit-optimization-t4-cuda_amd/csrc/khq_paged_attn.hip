@@ -16,6 +16,7 @@
 #include "khq_paged_internal.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace khq {
 namespace paged {
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
     x8 qf[KS];
 #pragma unroll
     for (int st = 0; st < KS; st++) qf[st] = *reinterpret_cast<const x8*>(&lds.q[li][32 * st + 8 * lg]);
-    const int vis = li < rows ? visible(a, it, r0 + li) : 0;
+    const int vis = visible(a, it, r0 + min(li, rows - 1));  // (no row: what the last one sees)
     const int vis_lo = visible(a, it, r0), vis_hi = visible(a, it, r0 + rows - 1);
     const int units = (vis_hi + STREAM_UNIT - 1) / STREAM_UNIT;
     const int t_lo = (int)((long long)units * it.split / it.n_split) * NW;
@@ -345,13 +346,11 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
             for (int e = 0; e < 8; e++)
                 if (bad_keys >> (16 * (e >> 2) + 4 * lg + (e & 3)) & 1) sc[e] = __builtin_nanf("");
         }
-        if (key0 + 32 > vis_lo || rows < 16) {  // (rows past the tile's see nothing)
+        bool odd = false;  // values that are no numbers where a row's mask has to hold
+        if (key0 + 32 > vis_lo) {
 #pragma unroll
             for (int e = 0; e < 8; e++)
                 if (key0 + 16 * (e >> 2) + 4 * lg + (e & 3) >= vis) sc[e] = -INFINITY;
-        }
-        bool odd = false;  // values that are no numbers where a row's mask has to hold
-        if (key0 + 32 > vis_lo) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const bool none = key0 + (j & 4) * 4 + 4 * lg + (j & 3) >= vis_hi;
@@ -518,83 +517,394 @@ __global__ __launch_bounds__(256) void attn_stream_join_kernel(AttnArgs a, Part 
     ((T*)a.r.out)[(it.row0 + tok) * a.r.out_token + hq * a.r.out_head + c] = (T)v;
 }
 
-// One wavefront a (row, head): the keys one after the other.
-template <typename T, int D>
-__global__ __launch_bounds__(64) void attn_row_kernel(AttnArgs a, Part pt) {
-    const khq_attn_rows& r = a.r;
-    const int row = blockIdx.x, hq = blockIdx.y, lane = threadIdx.x;
-    int lo = 0, hi = r.n_seq;  // the last sequence whose first row is not past row
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (r.cu_q[mid] <= row) lo = mid;
-        else hi = mid;
+// ------------------------------------------------------------ many rows
+typedef __attribute__((address_space(3))) char lds_char;
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+    return (uint32_t)(uintptr_t)(lds_char*)p;
+}
+// 16 bytes a lane from g into LDS at to + 16 lane, past the registers.  (Not the
+// builtin: behind it the compiler waits for the load before every LDS read.)
+__device__ __forceinline__ void load_lds16(const void* g, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g),
+                 "s"(__builtin_amdgcn_readfirstlane(to))
+                 : "memory");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Four keys' values of a lane's dim: each 16 lanes read a 4 x 16 block whose
+// row j lies at lanes 4 j .. 4 j + 3, and lane i gets its column i.
+__device__ __forceinline__ u2 read_tr(const char* p) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                      (__attribute__((address_space(3))) s4*)p));
+}
+
+constexpr int TAB = 2048;  // block table entries in LDS
+
+// Row r of the item: its output, times the gate, four dims from dim on.
+template <typename T>
+__device__ __forceinline__ void store_row4(const AttnArgs& a, const Item& it, int r, int dim, f4 o) {
+    const int tok = a.by_rep.div(r), hq = it.head * a.n_rep + r - tok * a.n_rep;
+    if (a.r.gate) {
+        const u2e g = *reinterpret_cast<const u2e*>((const T*)a.r.gate + (it.row0 + tok) * a.r.gate_token +
+                                                    hq * a.r.gate_head + dim);
+        const typename V<T>::x4 gv = __builtin_bit_cast(typename V<T>::x4, u2{g.x, g.y});
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] *= sigmoid(gv[e]);
     }
-    const int first = r.cu_q[lo], end = r.cu_q[lo + 1];
-    if (row < first || row >= end) return;
-    if (pt.serve == SERVE_LARGE && (end - first) * a.n_rep <= SMALL_ROWS) return;
-    const long long cap = (long long)r.table_ld * a.p.page_size;
-    const int kv = (int)min((long long)max(r.seq_kv[lo], 0), cap);
-    const int vis = min(kv, kv - (end - first) + (row - first) + 1);
-    constexpr int N = D / 64;
-    float q[N], acc[N], m = -INFINITY, l = 0.f;
-    const int h = hq / a.n_rep;
-    for (int i = 0; i < N; i++) {
-        q[i] = (float)((const T*)r.q)[row * r.q_token + hq * r.q_head + lane * N + i] * r.scale;
-        acc[i] = 0.f;
-    }
-    for (int k = 0; k < vis; k++) {
-        const int page = r.table[(size_t)lo * r.table_ld + k / a.p.page_size];
-        if ((unsigned)page >= (unsigned)a.p.n_pages) {
-            l = NAN;
-            continue;
+    *reinterpret_cast<u2e*>((T*)a.r.out + (it.row0 + tok) * a.r.out_token + hq * a.r.out_head + dim) =
+        u2e{pack<T>(o[0], o[1]), pack<T>(o[2], o[3])};
+}
+
+// 32 rows a wavefront on 32x32x16 MFMAs, 64 keys and values at a time in one of
+// two LDS slots while the next ones are on their way into the other, straight
+// from memory.  KG 1: eight wavefronts of 256 rows, each taking all 64 keys; KG
+// 2: 128 rows, each wavefront 32 of the 64 keys of its rows, the two halves
+// joined at the end.  S^T = K Q^T: its result (row = lane % 32, key 8 (e / 4) +
+// 4 (lane / 32) + e % 4 in register e) is the B operand of O^T += V^T P^T when
+// that product's K index i of step s stands for key 16 s + 8 (i / 4) + 4 (lane /
+// 32) + i % 4, which is how V is read, transposed on its way out of LDS.
+// 16-byte pieces of a row are permuted (K: piece ^ key, V: piece ^ 4 key) so
+// that the lanes of a read meet all banks.
+template <typename T, int D, int KG>
+__global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) {
+    constexpr int NS = D / 16, ND = D / 32;  // K steps of a score, dim tiles
+    constexpr int ROW = 2 * D, SLOT = 64 * ROW;  // bytes
+    constexpr int CH = D / 8, KPI = 64 / CH, NI = 64 / KPI / 8;  // pieces a row, keys a load, loads
+    typedef typename V<T>::x8 x8;
+    extern __shared__ __align__(1024) char lds[];
+    char* const ks = lds;
+    char* const vs = lds + 2 * SLOT;
+    int* const tab = reinterpret_cast<int*>(lds + 4 * SLOT);
+    __shared__ int s_bad;
+    __shared__ float s_m[4][32], s_l[4][32];
+    Item it;
+    if (!schedule(a, pt, blockIdx.x, false, it)) return;
+    const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int ln = lane & 31, hh = lane >> 5;
+    const int rg = KG == 1 ? wv : wv & 3, kg = KG == 1 ? 0 : wv >> 2;
+    constexpr int BR = 256 / KG;
+    const int n_rows = it.n_q * a.n_rep;
+    const int r = it.qt * BR + rg * 32 + ln;
+    const bool r_ok = r < n_rows;
+    // (a lane of no row sees what the last row sees and stores nothing)
+    const int vis = visible(a, it, min(r, n_rows - 1));
+    const int vis_hi = visible(a, it, min(it.qt * BR + BR, n_rows) - 1);
+    const int units = (vis_hi + 63) >> 6;
+    const int u_lo = (int)((long long)units * it.split / it.n_split);
+    const int u_hi = (int)((long long)units * (it.split + 1) / it.n_split);
+    x8 qb[NS];
+    {
+        const uint32_t flip = a.r.scale < 0.0f ? 0x80008000u : 0u;
+        const int rr = min(r, n_rows - 1), tok = a.by_rep.div(rr);
+        const T* q = (const T*)a.r.q + (it.row0 + tok) * a.r.q_token +
+                     (it.head * a.n_rep + rr - tok * a.n_rep) * a.r.q_head + 8 * hh;
+#pragma unroll
+        for (int st = 0; st < NS; st++) {
+            const u4e v = *reinterpret_cast<const u4e*>(q + 16 * st);
+            qb[st] = __builtin_bit_cast(x8, u4{v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip});
         }
-        const long long at = page * a.p.page_stride + k % a.p.page_size * a.p.token_stride +
-                             h * a.p.head_stride + lane * N;
-        float s = 0.f;
-        for (int i = 0; i < N; i++) s += q[i] * (float)((const T*)a.p.k)[at + i];
-        for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
-        const float mn = fmaxf(m, s);
-        const float f = m == mn ? 1.f : expf(m - mn), p = expf(s - mn);
-        m = mn;
-        l = l * f + p;
-        for (int i = 0; i < N; i++) acc[i] = acc[i] * f + p * (float)((const T*)a.p.v)[at + i];
     }
-    for (int i = 0; i < N; i++) {
-        float o = vis > 0 ? acc[i] / l : 0.f;
-        if (r.gate)
-            o /= 1.f + expf(-(float)((const T*)r.gate)[row * r.gate_token + hq * r.gate_head + lane * N + i]);
-        ((T*)r.out)[row * r.out_token + hq * r.out_head + lane * N + i] = (T)o;
+    const float sc2 = score_scale(a.r.scale);
+    int w0 = 0;  // first page of the table's window
+    auto fill = [&](int u) {
+        w0 = a.by_page.div(u * 64);
+        const int n = min(TAB, a.by_page.div(vis_hi - 1) + 1 - w0);
+        for (int i = tid; i < n; i += 512) {
+            const int e = a.r.table[(size_t)it.seq * a.r.table_ld + w0 + i];
+            const bool bad = (unsigned)e >= (unsigned)a.p.n_pages;
+            tab[i] = bad ? -1 : e;
+            if (bad) s_bad = 1;
+        }
+    };
+    auto stage = [&](int u, int slot) {
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int key = (wv * NI + i) * KPI + lane / CH, p = lane % CH;
+            const int t = min(u * 64 + key, vis_hi - 1);
+            const int pg = a.by_page.div(t);
+            const long long off = max(tab[pg - w0], 0) * a.p.page_stride +
+                                  (t - pg * a.p.page_size) * a.p.token_stride + it.head * a.p.head_stride;
+            const int fk = D == 64 ? (key >> 1) & 7 : key & 15;
+            const int fv = D == 64 ? (key & 2) << 1 : (key & 3) << 2;
+            load_lds16((const T*)a.p.k + off + 8 * (p ^ fk), lds_addr(ks) + slot * SLOT + (wv * NI + i) * 1024);
+            load_lds16((const T*)a.p.v + off + 8 * (p ^ fv), lds_addr(vs) + slot * SLOT + (wv * NI + i) * 1024);
+        }
+    };
+    f16v acc[ND];
+#pragma unroll
+    for (int i = 0; i < ND; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[i][e] = 0.0f;
+    float m_ref = M_NONE, l_part = 0.0f;
+    // where a lane's operands lie in a slot's 32 keys
+    const int k_at = ln * ROW + ((hh ^ (D == 64 ? (ln >> 1) & 7 : ln & 15)) << 4);
+    const int vj = (lane >> 2) & 3;
+    const int v_at = (4 * hh + vj) * ROW + ((D == 64 ? vj >> 1 : vj) << 6) +
+                     (2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8;
+    if (tid == 0) s_bad = 0;
+    __syncthreads();
+    if (u_lo < u_hi) {
+        fill(u_lo);
+        __syncthreads();
+        stage(u_lo, 0);
     }
+    // unit u is waited for, the next one started
+    auto begin = [&](int u) {
+        wait_loads();
+        __syncthreads();  // u is there, u - 1 is done with
+        if (u + 1 < u_hi) {
+            if (a.by_page.div(min(u * 64 + 127, vis_hi - 1)) - w0 >= TAB) {
+                fill(u);
+                __syncthreads();
+            }
+            stage(u + 1, (u + 1 - u_lo) & 1);
+        }
+    };
+    auto keys = [&](int u, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+#pragma unroll 1
+        for (int sub = kg; sub < 2; sub += KG) {
+            const int key0 = u * 64 + 32 * sub;
+            if (MASKED && __ballot(vis > key0) == 0ull) break;  // these keys are no row's
+            const int at = ((u - u_lo) & 1) * SLOT + sub * 32 * ROW;
+            const char* const kb = ks + at;
+            const char* const vb = vs + at;
+            // (opaque: the permuted places are a xor each, and would be kept in
+            // registers that there are not)
+            int ka = k_at, va = v_at;
+            asm("" : "+v"(ka), "+v"(va));
+            f16v s2[2];
+#pragma unroll
+            for (int e = 0; e < 16; e++) s2[0][e] = s2[1][e] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < NS; st++)
+                s2[st & 1] = mfma32(*reinterpret_cast<const x8*>(kb + (ka ^ (st << 5))), qb[st], s2[st & 1]);
+            float sc[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) sc[e] = s2[0][e] + s2[1][e];
+            bool odd = false;  // values that are no numbers where a row's mask has to hold
+            if constexpr (MASKED) {
+                if (s_bad) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int t = min(key0 + 8 * (e >> 2) + 4 * hh + (e & 3), vis_hi - 1);
+                        if (tab[a.by_page.div(t) - w0] < 0) sc[e] = __builtin_nanf("");
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (key0 + 8 * (e >> 2) + 4 * hh + (e & 3) >= vis) sc[e] = -INFINITY;
+                for (int i = 0; i < D / 16; i++) {
+                    const u4 v = *reinterpret_cast<const u4*>(vb + (i * 64 + lane) * 16);
+                    odd = odd || nonfinite_pair<T>(v.x) || nonfinite_pair<T>(v.y) ||
+                          nonfinite_pair<T>(v.z) || nonfinite_pair<T>(v.w);
+                }
+                odd = __ballot(odd) != 0ull;
+            }
+            float lmax = sc[0];
+#pragma unroll
+            for (int e = 1; e < 16; e++) lmax = fmaxf(lmax, sc[e]);
+            lmax *= sc2;
+            if (__ballot(lmax > m_ref + GAP) != 0ull) {
+                lmax = fmaxf(lmax, __shfl_xor(lmax, 32, 64));
+                const float m_new = fmaxf(m_ref, lmax);
+                const float fac = __builtin_amdgcn_exp2f(m_ref - m_new);  // 0 from M_NONE, 1 where it stays
+                m_ref = m_new;
+                l_part *= fac;
+#pragma unroll
+                for (int i = 0; i < ND; i++) acc[i] *= fac;
+            }
+            uint32_t pw[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                pw[e] = pack<T>(__builtin_amdgcn_exp2f(fmaf(sc[2 * e], sc2, -m_ref)),
+                                __builtin_amdgcn_exp2f(fmaf(sc[2 * e + 1], sc2, -m_ref)));
+                l_part = add_pair<T>(pw[e], l_part);
+            }
+            x8 pb[2];
+#pragma unroll
+            for (int sp = 0; sp < 2; sp++)
+                pb[sp] = __builtin_bit_cast(x8, u4{pw[4 * sp], pw[4 * sp + 1], pw[4 * sp + 2], pw[4 * sp + 3]});
+            if (MASKED && odd) {
+                // 0 * inf is no 0: such values join the rows that see them apart
+#pragma unroll 1
+                for (int k = 0; k < 32; k++) {
+                    const int fv = D == 64 ? (k & 2) << 1 : (k & 3) << 2;
+                    const bool sees = key0 + k < vis;
+#pragma unroll
+                    for (int i = 0; i < ND; i++)
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const u2 w = *reinterpret_cast<const u2*>(vb + k * ROW + ((4 * i + q) ^ fv) * 16 + hh * 8);
+                            const typename V<T>::x4 v = __builtin_bit_cast(typename V<T>::x4, w);
+#pragma unroll
+                            for (int c = 0; c < 4; c++) {
+                                const float x = (float)v[c];
+                                acc[i][4 * q + c] += sees && !(fabsf(x) < INFINITY) ? x : 0.0f;
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < ND; i++)
+#pragma unroll
+                for (int sp = 0; sp < 2; sp++) {
+                    const char* const p = vb + (va ^ (i << 6)) + 16 * sp * ROW;
+                    u2 lo = read_tr(p), hi = read_tr(p + 8 * ROW);
+                    if (MASKED && odd) {  // ... and leave the product
+                        lo = u2{finite_pair<T>(lo.x), finite_pair<T>(lo.y)};
+                        hi = u2{finite_pair<T>(hi.x), finite_pair<T>(hi.y)};
+                    }
+                    acc[i] = mfma32(__builtin_bit_cast(x8, u4{lo.x, lo.y, hi.x, hi.y}), pb[sp], acc[i]);
+                }
+        }
+    };
+    // units that every row sees whole, then the others; all from the first entry
+    // outside the cache on
+    const int u_mid = min(u_hi, visible(a, it, it.qt * BR) >> 6);
+    int u = u_lo;
+    bool begun = false;
+    for (; u < u_mid; u++) {
+        begin(u);
+        if ((begun = s_bad != 0)) break;
+        keys(u, std::false_type{});
+    }
+    for (; u < u_hi; u++) {
+        if (!begun) begin(u);
+        begun = false;
+        keys(u, std::true_type{});
+    }
+    float l_row = l_part + __shfl_xor(l_part, 32, 64);
+    if constexpr (KG == 2) {  // the other half of the keys
+        __syncthreads();
+        f4* const x = reinterpret_cast<f4*>(lds) + rg * (ND * 4 * 64) + lane;
+        if (kg == 1) {
+#pragma unroll
+            for (int i = 0; i < ND; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    x[(i * 4 + q) * 64] = f4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
+            if (hh == 0) {
+                s_m[rg][ln] = m_ref;
+                s_l[rg][ln] = l_row;
+            }
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const float m2 = s_m[rg][ln], m = fmaxf(m_ref, m2);
+        const float f1 = __builtin_amdgcn_exp2f(m_ref - m), f2 = __builtin_amdgcn_exp2f(m2 - m);
+        m_ref = m;
+        l_row = l_row * f1 + s_l[rg][ln] * f2;
+#pragma unroll
+        for (int i = 0; i < ND; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const f4 o = x[(i * 4 + q) * 64];
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[i][4 * q + c] = acc[i][4 * q + c] * f1 + o[c] * f2;
+            }
+    }
+    // ---- dims 32 i + 8 q + 4 hh + c of row r
+    if (it.n_split == 1) {
+        if (!r_ok) return;
+        const float inv = vis > 0 ? 1.0f / l_row : 0.0f;
+#pragma unroll
+        for (int i = 0; i < ND; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                store_row4<T>(a, it, r, 32 * i + 8 * q + 4 * hh,
+                              f4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]} * inv);
+    } else {
+        float* ws = static_cast<float*>(a.r.ws);
+        const int block = it.block + it.split * a.p.H_kv;
+        f4* const x = reinterpret_cast<f4*>(part_acc(ws, pt, D, block)) + rg * (ND * 4 * 64) + lane;
+#pragma unroll
+        for (int i = 0; i < ND; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                x[(i * 4 + q) * 64] = f4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
+        if (hh == 0) part_ml(ws, pt, D, block)[rg * 32 + ln] = float2{m_ref, l_row};
+    }
+}
+
+// The splits of 32 rows, a wavefront 32 dims of them.
+template <typename T, int D>
+__global__ __launch_bounds__(2 * D) void attn_tile_join_kernel(AttnArgs a, Part pt) {
+    constexpr int ND = D / 32;
+    const int groups = pt.rows / 32;
+    Item it;
+    if (!schedule(a, pt, blockIdx.x / groups, true, it)) return;
+    const int rg = blockIdx.x % groups;
+    const int i = threadIdx.x >> 6, lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5;
+    const int r = it.qt * pt.rows + rg * 32 + ln, h_kv = a.p.H_kv;
+    if (it.qt * pt.rows + rg * 32 >= it.n_q * a.n_rep) return;
+    float* ws = static_cast<float*>(a.r.ws);
+    float m = M_NONE, l = 0.0f;
+    for (int s = 0; s < it.n_split; s++)
+        m = fmaxf(m, part_ml(ws, pt, D, it.block + s * h_kv)[rg * 32 + ln].x);
+    f4 o[4] = {};
+#pragma unroll 4
+    for (int s = 0; s < it.n_split; s++) {
+        const float2 ml = part_ml(ws, pt, D, it.block + s * h_kv)[rg * 32 + ln];
+        const f4* x = reinterpret_cast<const f4*>(part_acc(ws, pt, D, it.block + s * h_kv)) +
+                      (rg * ND + i) * (4 * 64) + lane;
+        const float f = __builtin_amdgcn_exp2f(ml.x - m);
+        l += ml.y * f;
+#pragma unroll
+        for (int q = 0; q < 4; q++) o[q] += x[q * 64] * f;
+    }
+    if (r >= it.n_q * a.n_rep) return;
+    const float inv = visible(a, it, r) > 0 ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int q = 0; q < 4; q++) store_row4<T>(a, it, r, 32 * i + 8 * q + 4 * hh, o[q] * inv);
 }
 
 // What a call of these sizes launches.
 struct Plan {
     bool stream, tile;
     Part ps, pl;
-    int stream_blocks;
+    int stream_blocks, tile_blocks, kg;
 };
 Plan plan_of(int n_tok, int n_seq, int H_q, int H_kv, int max_q) {
-    const int n_rep = H_q / H_kv;
+    const int n_rep = H_q / H_kv, seqs = std::min(n_tok, n_seq);
+    const long long rows = (long long)n_tok * n_rep;
     Plan p{};
     p.stream = true;  // there may be short sequences whatever max_q says
     p.tile = (long long)max_q * n_rep > SMALL_ROWS;
     p.ps = Part{16, STREAM_UNIT, STREAM_SLOTS, p.tile ? SERVE_SMALL : SERVE_ALL, true};
-    p.pl = Part{0, 0, 0, SERVE_LARGE, false};
     // row tiles there may be: those served hold 16 rows or, served all, n_tok's
-    const long long most = p.tile ? (long long)std::min(n_tok, n_seq) * H_kv
-                                  : ((long long)n_tok * n_rep / 16 + std::min(n_tok, n_seq)) * H_kv;
+    const long long most = p.tile ? (long long)seqs * H_kv : (rows / 16 + seqs) * H_kv;
     p.stream_blocks = (int)std::max<long long>(STREAM_SLOTS, most);
+    p.kg = rows / 256 * H_kv >= TILE_SLOTS ? 1 : 2;
+    const int br = 256 / p.kg;
+    p.pl = Part{br, TILE_UNIT, TILE_SLOTS, SERVE_LARGE, rows / br * H_kv < TILE_SLOTS};
+    p.tile_blocks = (int)std::max<long long>(p.pl.split ? TILE_SLOTS : 0, (rows / br + seqs) * H_kv);
     return p;
 }
 size_t part_bytes(const Part& pt, int d) {
-    return (size_t)pt.slots * pt.rows * (d * sizeof(float) + sizeof(float2));
+    return pt.split ? (size_t)pt.slots * pt.rows * (d * sizeof(float) + sizeof(float2)) : 0;
+}
+
+template <typename T, int D, int KG>
+hipError_t launch_tile(const AttnArgs& a, const Plan& p, hipStream_t st) {
+    constexpr int bytes = 4 * 64 * 2 * D + TAB * (int)sizeof(int);
+    const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(attn_tile_kernel<T, D, KG>), bytes);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((attn_tile_kernel<T, D, KG>), dim3(p.tile_blocks), dim3(512), bytes, st, a, p.pl);
+    if (p.pl.split)
+        hipLaunchKernelGGL((attn_tile_join_kernel<T, D>), dim3(TILE_SLOTS * (p.pl.rows / 32)), dim3(2 * D), 0,
+                           st, a, p.pl);
+    return hipGetLastError();
 }
 
 template <typename T, int D>
 hipError_t launch(const AttnArgs& a, hipStream_t st) {
     const Plan p = plan_of(a.r.n_tok, a.r.n_seq, a.r.H_q, a.p.H_kv, a.r.max_q);
-    if (p.tile)
-        hipLaunchKernelGGL((attn_row_kernel<T, D>), dim3(a.r.n_tok, a.r.H_q), dim3(64), 0, st, a, p.pl);
+    if (p.tile) {
+        const hipError_t e = p.kg == 1 ? launch_tile<T, D, 1>(a, p, st) : launch_tile<T, D, 2>(a, p, st);
+        if (e != hipSuccess) return e;
+    }
     if (p.stream) {
         hipLaunchKernelGGL((attn_stream_kernel<T, D>), dim3(p.stream_blocks), dim3(64 * STREAM_WAVES), 0,
                            st, a, p.ps);
