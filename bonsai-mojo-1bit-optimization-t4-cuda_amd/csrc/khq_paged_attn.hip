@@ -476,45 +476,50 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
     }
 }
 
-// The splits of one row: each wavefront sums every fourth, the four meet in LDS.
-template <typename T, int D>
+// The splits of a row: W wavefronts sum every W-th and meet in LDS.
+template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void attn_stream_join_kernel(AttnArgs a, Part pt) {
-    constexpr int E = D / 64;
-    __shared__ float s_o[4][D], s_l[4];
+    constexpr int E = D / 64, RB = 4 / W;  // dims a lane, rows a block
+    typedef float fe __attribute__((ext_vector_type(E)));
+    __shared__ float s_o[W > 1 ? W : 1][D], s_l[4];
     Item it;
-    if (!schedule(a, pt, blockIdx.x >> 4, true, it)) return;
-    const int row = blockIdx.x & 15, r = it.qt * 16 + row;
-    if (r >= it.n_q * a.n_rep) return;
+    if (!schedule(a, pt, blockIdx.x / (16 / RB), true, it)) return;
     const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, h_kv = a.p.H_kv;
+    const int row = blockIdx.x % (16 / RB) * RB + wv / W, r = it.qt * 16 + row;
+    if (r >= it.n_q * a.n_rep) return;  // (W > 1: of the whole block)
     float* ws = static_cast<float*>(a.r.ws);
     float m = M_NONE;
     for (int i = lane; i < it.n_split; i += 64)
         m = fmaxf(m, part_ml(ws, pt, D, it.block + i * h_kv)[row].x);
 #pragma unroll
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    float o[E] = {}, l = 0.0f;
-#pragma unroll 4
-    for (int i = wv; i < it.n_split; i += 4) {
+    fe o = {};
+    float l = 0.0f;
+#pragma unroll 8
+    for (int i = wv % W; i < it.n_split; i += W) {
         const float2 ml = part_ml(ws, pt, D, it.block + i * h_kv)[row];
-        const float* acc = part_acc(ws, pt, D, it.block + i * h_kv) + row * D + E * lane;
+        const fe x = *reinterpret_cast<const fe*>(part_acc(ws, pt, D, it.block + i * h_kv) + row * D + E * lane);
         const float f = __builtin_amdgcn_exp2f(ml.x - m);
         l += ml.y * f;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] += acc[e] * f;
+        o += x * f;
     }
+    if constexpr (W > 1) {
 #pragma unroll
-    for (int e = 0; e < E; e++) s_o[wv][E * lane + e] = o[e];
-    if (lane == 0) s_l[wv] = l;
-    __syncthreads();
-    const int c = threadIdx.x;
-    if (c >= D) return;
-    float v = (s_o[0][c] + s_o[1][c]) + (s_o[2][c] + s_o[3][c]);
-    l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+        for (int e = 0; e < E; e++) s_o[wv][E * lane + e] = o[e];
+        if (lane == 0) s_l[wv] = l;
+        __syncthreads();
+        if (wv > 0) return;
+        l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            o[e] = (s_o[0][E * lane + e] + s_o[1][E * lane + e]) + (s_o[2][E * lane + e] + s_o[3][E * lane + e]);
+    }
     const int tok = a.by_rep.div(r), hq = it.head * a.n_rep + r - tok * a.n_rep;
-    v *= visible(a, it, r) > 0 ? 1.0f / l : 0.0f;
-    if (a.r.gate)
-        v *= sigmoid(((const T*)a.r.gate)[(it.row0 + tok) * a.r.gate_token + hq * a.r.gate_head + c]);
-    ((T*)a.r.out)[(it.row0 + tok) * a.r.out_token + hq * a.r.out_head + c] = (T)v;
+    const float inv = visible(a, it, r) > 0 ? 1.0f / l : 0.0f;
+    const T* gate = (const T*)a.r.gate + (it.row0 + tok) * a.r.gate_token + hq * a.r.gate_head + E * lane;
+    T* out = (T*)a.r.out + (it.row0 + tok) * a.r.out_token + hq * a.r.out_head + E * lane;
+#pragma unroll
+    for (int e = 0; e < E; e++) out[e] = (T)(o[e] * inv * (a.r.gate ? sigmoid(gate[e]) : 1.0f));
 }
 
 // ------------------------------------------------------------ many rows
@@ -864,7 +869,7 @@ __global__ __launch_bounds__(2 * D) void attn_tile_join_kernel(AttnArgs a, Part 
 struct Plan {
     bool stream, tile;
     Part ps, pl;
-    int stream_blocks, tile_blocks, kg;
+    int stream_blocks, stream_joins, tile_blocks, tile_joins, kg;
 };
 Plan plan_of(int n_tok, int n_seq, int H_q, int H_kv, int max_q) {
     const int n_rep = H_q / H_kv, seqs = std::min(n_tok, n_seq);
@@ -876,10 +881,13 @@ Plan plan_of(int n_tok, int n_seq, int H_q, int H_kv, int max_q) {
     // row tiles there may be: those served hold 16 rows or, served all, n_tok's
     const long long most = p.tile ? (long long)seqs * H_kv : (rows / 16 + seqs) * H_kv;
     p.stream_blocks = (int)std::max<long long>(STREAM_SLOTS, most);
+    p.stream_joins = (int)std::min<long long>(STREAM_SLOTS, most);
     p.kg = rows / 256 * H_kv >= TILE_SLOTS ? 1 : 2;
     const int br = 256 / p.kg;
     p.pl = Part{br, TILE_UNIT, TILE_SLOTS, SERVE_LARGE, rows / br * H_kv < TILE_SLOTS};
-    p.tile_blocks = (int)std::max<long long>(p.pl.split ? TILE_SLOTS : 0, (rows / br + seqs) * H_kv);
+    const long long tiles = (rows / br + seqs) * H_kv;
+    p.tile_blocks = (int)std::max<long long>(p.pl.split ? TILE_SLOTS : 0, tiles);
+    p.tile_joins = (int)std::min<long long>(TILE_SLOTS, tiles);
     return p;
 }
 size_t part_bytes(const Part& pt, int d) {
@@ -893,8 +901,8 @@ hipError_t launch_tile(const AttnArgs& a, const Plan& p, hipStream_t st) {
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((attn_tile_kernel<T, D, KG>), dim3(p.tile_blocks), dim3(512), bytes, st, a, p.pl);
     if (p.pl.split)
-        hipLaunchKernelGGL((attn_tile_join_kernel<T, D>), dim3(TILE_SLOTS * (p.pl.rows / 32)), dim3(2 * D), 0,
-                           st, a, p.pl);
+        hipLaunchKernelGGL((attn_tile_join_kernel<T, D>), dim3(p.tile_joins * (p.pl.rows / 32)), dim3(2 * D),
+                           0, st, a, p.pl);
     return hipGetLastError();
 }
 
@@ -908,8 +916,14 @@ hipError_t launch(const AttnArgs& a, hipStream_t st) {
     if (p.stream) {
         hipLaunchKernelGGL((attn_stream_kernel<T, D>), dim3(p.stream_blocks), dim3(64 * STREAM_WAVES), 0,
                            st, a, p.ps);
-        hipLaunchKernelGGL((attn_stream_join_kernel<T, D>), dim3(STREAM_SLOTS * 16), dim3(256), 0, st, a,
-                           p.ps);
+        // few rows of many splits: a block a row (one sequence of 512 tokens and 24 / 4
+        // heads ...), else a wavefront a row
+        if (p.stream_joins <= 32)
+            hipLaunchKernelGGL((attn_stream_join_kernel<T, D, 4>), dim3(p.stream_joins * 16), dim3(256), 0, st,
+                               a, p.ps);
+        else
+            hipLaunchKernelGGL((attn_stream_join_kernel<T, D, 1>), dim3(p.stream_joins * 4), dim3(256), 0, st, a,
+                               p.ps);
     }
     return hipGetLastError();
 }

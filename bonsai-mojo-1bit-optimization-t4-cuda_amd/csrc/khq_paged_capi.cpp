@@ -40,10 +40,12 @@ int khq_paged_plan(const int* q_len, const int* kv_len, int* table, int table_ld
         !state_out || !status || n_seq <= 0 || n_seq > KHQ_PAGED_MAX_SEQ || table_ld <= 0 ||
         n_pages <= 0 || page_size <= 0 || n_tok < 0 || (n_tok > 0 && (!positions || !slots)))
         return -100;
+    if (n_pages >= 1 << 30 || n_tok >= 1 << 30) return -100;  // sums of two stay in 32 bits
     if ((long long)n_pages * page_size > 0x7fffffffLL || (long long)table_ld * page_size > 0x7fffffffLL)
         return -100;
     khq::paged::PlanArgs a{q_len, kv_len, table, free_pages, state, cu_q, seq_kv, kv_out, state_out,
-                           status, positions, slots, n_seq, table_ld, n_pages, page_size, n_tok};
+                           status, positions, slots, n_seq, table_ld, n_pages, page_size, n_tok,
+                           khq::FastDiv(page_size)};
     return rc_of(khq::paged::launch_plan(a, kv_out == kv_len || state_out == state, stream));
 }
 
@@ -63,7 +65,10 @@ int khq_qk_norm_rope(const khq_rows* rows, const khq_pages* pages, hipStream_t s
     if (r.n == 0) return 0;
     khq::paged::RowsArgs a{};
     a.r = r;
-    if (pages) a.p = *pages;
+    if (pages) {
+        a.p = *pages;
+        a.by_page = khq::FastDiv(pages->page_size);
+    }
     // revolutions a position of each pair, in 64 bits: a table of the last base and width
     static thread_local double freq[128], base = 0;
     static thread_local int width = 0;

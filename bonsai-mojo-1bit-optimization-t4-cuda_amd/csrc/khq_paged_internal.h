@@ -26,6 +26,7 @@ struct PlanArgs {
     const int* state;
     int *cu_q, *seq_kv, *kv_out, *state_out, *status, *positions, *slots;
     int n_seq, table_ld, n_pages, page_size, n_tok;
+    FastDiv by_page;  // page_size
 };
 // in_place: kv_out is kv_len or state_out is state.
 hipError_t launch_plan(const PlanArgs& a, bool in_place, hipStream_t st);
@@ -33,6 +34,7 @@ hipError_t launch_plan(const PlanArgs& a, bool in_place, hipStream_t st);
 struct RowsArgs {
     khq_rows r;
     khq_pages p;        // k = NULL: none
+    FastDiv by_page;    // page_size
     double freq[128];   // revolutions a position, of each dim pair
 };
 hipError_t launch_rows(const RowsArgs& a, hipStream_t st);

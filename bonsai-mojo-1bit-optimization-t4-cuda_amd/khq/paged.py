@@ -39,6 +39,8 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _HEAD_DIMS = (64, 128, 256)
 
 _paged = None
+# the raw handle of a device's current stream, where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def lib() -> ctypes.CDLL:
@@ -63,84 +65,113 @@ def _call(name: str, *args, check: bool = True) -> int:
     return rc
 
 
-def _i32(t, shape, name: str, device) -> int:
-    """Pointer of an int32 tensor of this shape (None: any length), contiguous."""
+def _i32(t, n: int, name: str, device: int) -> int:
+    """Pointer of a contiguous int32 tensor of n elements on this device."""
+    if (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == device
+            and t.numel() == n and t.is_contiguous()):
+        return t.data_ptr()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
     if t.dtype != torch.int32:
         raise TypeError(f"{name}: dtype {t.dtype}, expected torch.int32")
-    if t.device != device:
-        raise ValueError(f"{name}: on {t.device}, expected {device}")
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: must be contiguous")
-    return t.data_ptr()
+    if t.get_device() != device:
+        raise ValueError(f"{name}: on {t.device}, expected cuda:{device}")
+    if t.numel() != n:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {n} elements")
+    raise ValueError(f"{name}: must be contiguous")
 
 
-def _heads(t, shape, dtype, name: str, device):
+def _table(t, n_seq, device: int):
+    """(pointer, rows, width) of a block table i32 [n_seq][pages]."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("table: expected a torch.Tensor")
+    shape = t.shape
+    if len(shape) != 2 or (n_seq is not None and shape[0] != n_seq) or not 0 < shape[0] <= MAX_SEQ:
+        raise ValueError(f"table: shape {tuple(shape)}, expected "
+                         f"[{n_seq or f'1 to {MAX_SEQ}'}][pages of a sequence]")
+    n, width = shape
+    return _i32(t, n * width, "table", device), n, width
+
+
+def _heads(t, shape, dtype, name: str, device: int):
     """(pointer, token stride, head stride) of a [tokens][heads][dims] tensor whose
     dims are dense; tokens and heads may be strided."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device
+            and t.shape == shape):
+        token, head, dim = t.stride()
+        if dim == 1:
+            return t.data_ptr(), token, head
+        raise ValueError(f"{name}: its last dim must be dense")
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
     if t.dtype != dtype:
         raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
-    if t.device != device:
-        raise ValueError(f"{name}: on {t.device}, expected {device}")
-    if t.shape != shape:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
-    token, head, dim = t.stride()
-    if dim != 1:
-        raise ValueError(f"{name}: its last dim must be dense")
-    return t.data_ptr(), token, head
+    if t.get_device() != device:
+        raise ValueError(f"{name}: on {t.device}, expected cuda:{device}")
+    raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
-def _written(t, name: str):
-    """Refuses an output whose rows share memory (an expanded tensor)."""
-    n, h, d = t.shape
-    token, head, _ = t.stride()
+def _written(at, shape, name: str):
+    """Refuses an output (pointer and strides `at`) whose rows share memory, as an expanded
+    tensor's do."""
+    _, token, head = at
+    n, h, d = shape
     # dims inside heads inside tokens, or inside tokens inside heads
+    if head >= d and token >= (h - 1) * head + d or token >= d and head >= (n - 1) * token + d:
+        return
     by_token = (h == 1 or head >= d) and (n == 1 or token >= (h - 1) * head + d)
     by_head = (n == 1 or token >= d) and (h == 1 or head >= (n - 1) * token + d)
-    if t.numel() and not (by_token or by_head):
+    if n * h * d and not (by_token or by_head):
         raise ValueError(f"{name}: its rows overlap")
 
 
-def _device(t, name: str) -> torch.device:
+def _device(t, name: str) -> int:
+    """Index of the current device, the tensor's."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
     if not t.is_cuda:
         raise ValueError(f"{name}: must be a device tensor")
-    if t.device.index != torch.cuda.current_device():
+    device = t.get_device()
+    if device != torch.cuda.current_device():
         raise ValueError(f"{name}: on {t.device}, but the current device is "
                          f"cuda:{torch.cuda.current_device()}")
-    return t.device
+    return device
 
 
-def _pages(k, v, device) -> tuple[bytes, torch.Size]:
-    """struct khq_pages of k, v [n_pages][page_size][H_kv][head_dim] (any strides, dims dense)."""
+def _stream(stream, device: int):
+    """Handle of the stream, or of the device's current one (null: None)."""
+    if stream is not None or _raw_stream is None:
+        return stream_handle(stream)
+    return _raw_stream(device) or None
+
+
+def _pages(k, v, device: int):
+    """struct khq_pages of k, v [n_pages][page_size][H_kv][head_dim] (any strides, dims dense)
+    and their shape."""
     for t, name in ((k, "k_pages"), (v, "v_pages")):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name}: expected a torch.Tensor")
-        if t.dtype not in _DTYPES:
-            raise TypeError(f"{name}: dtype {t.dtype}, expected float16 or bfloat16")
-        if t.device != device:
-            raise ValueError(f"{name}: on {t.device}, expected {device}")
-    if k.dim() != 4 or k.shape[3] not in _HEAD_DIMS or 0 in k.shape:
-        raise ValueError(f"k_pages: shape {tuple(k.shape)}, expected "
+        if t.get_device() != device:
+            raise ValueError(f"{name}: on {t.device}, expected cuda:{device}")
+    dtype = _DTYPES.get(k.dtype)
+    if dtype is None:
+        raise TypeError(f"k_pages: dtype {k.dtype}, expected float16 or bfloat16")
+    shape = k.shape
+    if len(shape) != 4 or shape[3] not in _HEAD_DIMS or 0 in shape:
+        raise ValueError(f"k_pages: shape {tuple(shape)}, expected "
                          "[pages][page_size][heads][64, 128 or 256]")
-    if v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype:
+    strides = k.stride()
+    if v.shape != shape or v.stride() != strides or v.dtype != k.dtype:
         raise ValueError("v_pages: shape, strides and dtype must be those of k_pages")
-    page, token, head, dim = k.stride()
+    page, token, head, dim = strides
     kp, vp = k.data_ptr(), v.data_ptr()
     if dim != 1 or (page | token | head) % 8 or (kp | vp) % 16:
         raise ValueError("k_pages, v_pages: dims must be dense, strides and pointers multiples of "
                          "16 bytes")
-    n_pages, page_size, h_kv, d = k.shape
+    n_pages, page_size, h_kv, d = shape
     if n_pages * page_size >= 1 << 31:
         raise ValueError("k_pages: 2^31 slots or more")
-    return PAGES_STRUCT.pack(kp, vp, page, token, head, n_pages, page_size, h_kv, d,
-                             _DTYPES[k.dtype]), k.shape
+    return PAGES_STRUCT.pack(kp, vp, page, token, head, n_pages, page_size, h_kv, d, dtype), shape
 
 
 def plan(q_len, kv_len, table, free_pages, state, *, page_size: int, cu_q, seq_kv, kv_out,
@@ -150,23 +181,22 @@ def plan(q_len, kv_len, table, free_pages, state, *, page_size: int, cu_q, seq_k
     [n_seq][pages], free_pages [n_pages] and state [2] (first free entry, free pages) are the
     cache's bookkeeping; kv_out and state_out may be kv_len and state."""
     device = _device(q_len, "q_len")
-    n_seq = q_len.shape[0] if q_len.dim() == 1 else -1
-    if not 0 < n_seq <= MAX_SEQ:
-        raise ValueError(f"q_len: shape {tuple(q_len.shape)}, expected [1 to {MAX_SEQ}]")
+    n_seq = q_len.numel()
+    table_p, _, width = _table(table, n_seq, device)
     if page_size <= 0:
         raise ValueError("page_size must be positive")
-    n = (n_seq,)
-    args = (_i32(q_len, n, "q_len", device), _i32(kv_len, n, "kv_len", device),
-            _i32(table, (n_seq, None), "table", device), table.shape[1],
-            _i32(free_pages, (None,), "free_pages", device), _i32(state, (2,), "state", device),
-            n_seq, free_pages.shape[0], page_size)
-    positions_p = _i32(positions, (None,), "positions", device)
-    n_tok = positions.shape[0]
-    return _call("khq_paged_plan", *args, n_tok, _i32(cu_q, (n_seq + 1,), "cu_q", device),
-                 _i32(seq_kv, n, "seq_kv", device), _i32(kv_out, n, "kv_out", device),
-                 _i32(state_out, (2,), "state_out", device), _i32(status, (1,), "status", device),
-                 positions_p, _i32(slots, (n_tok,), "slots", device),
-                 stream_handle(stream), check=check)
+    for t, name in ((free_pages, "free_pages"), (positions, "positions")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a torch.Tensor")
+    n_pages, n_tok = free_pages.numel(), positions.numel()
+    return _call("khq_paged_plan", _i32(q_len, n_seq, "q_len", device),
+                 _i32(kv_len, n_seq, "kv_len", device), table_p, width,
+                 _i32(free_pages, n_pages, "free_pages", device), _i32(state, 2, "state", device),
+                 n_seq, n_pages, page_size, n_tok, _i32(cu_q, n_seq + 1, "cu_q", device),
+                 _i32(seq_kv, n_seq, "seq_kv", device), _i32(kv_out, n_seq, "kv_out", device),
+                 _i32(state_out, 2, "state_out", device), _i32(status, 1, "status", device),
+                 _i32(positions, n_tok, "positions", device), _i32(slots, n_tok, "slots", device),
+                 _stream(stream, device), check=check)
 
 
 def qk_norm_rope(q, k, q_out, *, positions=None, pos0: int = 0, q_weight=None, k_weight=None,
@@ -193,20 +223,20 @@ def qk_norm_rope(q, k, q_out, *, positions=None, pos0: int = 0, q_weight=None, k
         h_q = q.shape[1]
         q_at = _heads(q, q.shape, dt, "q", device)
         q_out_at = _heads(q_out, q.shape, dt, "q_out", device)
-        _written(q_out, "q_out")
+        _written(q_out_at, q.shape, "q_out")
     if k is not None:
         h_kv = k.shape[1] if k.dim() == 3 else 0
         k_at = _heads(k, (n, h_kv, d), dt, "k", device)
         if k_out is not None:
             k_out_at = _heads(k_out, k.shape, dt, "k_out", device)
-            _written(k_out, "k_out")
+            _written(k_out_at, k.shape, "k_out")
         if k_normed is not None:
             k_normed_at = _heads(k_normed, k.shape, dt, "k_normed", device)
-            _written(k_normed, "k_normed")
+            _written(k_normed_at, k.shape, "k_normed")
     for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None and (w.dtype != torch.float32 or w.shape != (d,) or w.device != device
-                              or not w.is_contiguous()):
-            raise ValueError(f"{name}: must be float32 [{d}] on {device}, contiguous")
+        if w is not None and (w.dtype != torch.float32 or w.shape != (d,)
+                              or w.get_device() != device or not w.is_contiguous()):
+            raise ValueError(f"{name}: must be float32 [{d}] on cuda:{device}, contiguous")
     pages, slots_p = None, 0
     if (k_pages is None) != (v_pages is None) or (k_pages is None) != (slots is None) or (
             k_pages is None) != (v is None):
@@ -218,10 +248,10 @@ def qk_norm_rope(q, k, q_out, *, positions=None, pos0: int = 0, q_weight=None, k
         if shape[2:] != (h_kv, d) or k_pages.dtype != dt:
             raise ValueError("k_pages: heads, width and dtype must be those of k")
         v_at = _heads(v, k.shape, dt, "v", device)
-        slots_p = _i32(slots, (n,), "slots", device)
+        slots_p = _i32(slots, n, "slots", device)
     elif k is not None and k_out is None and k_normed is None:
         raise ValueError("keys without k_out, k_normed or pages")
-    pos_p = _i32(positions, (n,), "positions", device) if positions is not None else 0
+    pos_p = _i32(positions, n, "positions", device) if positions is not None else 0
     if n == 0:  # (empty tensors have no address)
         return 0
     rows = ROWS_STRUCT.pack(
@@ -229,7 +259,7 @@ def qk_norm_rope(q, k, q_out, *, positions=None, pos0: int = 0, q_weight=None, k
         ptr(k_weight) or 0, pos_p, slots_p, *q_at[1:], *q_out_at[1:], *k_at[1:], *k_out_at[1:],
         *k_normed_at[1:], *v_at[1:], theta, eps, n, h_q, h_kv, d, rotary_dim, pos0,
         1 if round_norm else 0, _DTYPES[dt])
-    return _call("khq_qk_norm_rope", rows, pages, stream_handle(stream), check=check)
+    return _call("khq_qk_norm_rope", rows, pages, _stream(stream, device), check=check)
 
 
 def attn(q, k_pages, v_pages, out, *, cu_q, seq_kv, table, max_q: int, scale: float, gate=None,
@@ -240,30 +270,29 @@ def attn(q, k_pages, v_pages, out, *, cu_q, seq_kv, table, max_q: int, scale: fl
     it says too low or high costs only time).  workspace: a device tensor of attn_ws_bytes
     bytes for calls that may run at once with others; None: the library's."""
     device = _device(q, "q")
-    pages, (_, page_size, h_kv, d) = _pages(k_pages, v_pages, device)
-    dt = k_pages.dtype
-    if q.dim() != 3 or q.shape[2] != d or q.shape[1] % h_kv or q.shape[1] == 0:
-        raise ValueError(f"q: shape {tuple(q.shape)}, expected [tokens][a multiple of {h_kv}][{d}]")
-    shape = q.shape
-    q_at, out_at = _heads(q, shape, dt, "q", device), _heads(out, shape, dt, "out", device)
-    _written(out, "out")
-    gate_at = _heads(gate, shape, dt, "gate", device) if gate is not None else (0, 0, 0)
-    n_seq = table.shape[0]
-    if not 0 < n_seq <= MAX_SEQ:
-        raise ValueError(f"table: {n_seq} rows, expected 1 to {MAX_SEQ}")
+    pages, (_, _, h_kv, d) = _pages(k_pages, v_pages, device)
+    dt, shape = k_pages.dtype, q.shape
+    if len(shape) != 3 or shape[2] != d or shape[1] % h_kv or shape[1] == 0:
+        raise ValueError(f"q: shape {tuple(shape)}, expected [tokens][a multiple of {h_kv}][{d}]")
+    q_p, q_token, q_head = _heads(q, shape, dt, "q", device)
+    out_at = out_p, out_token, out_head = _heads(out, shape, dt, "out", device)
+    _written(out_at, shape, "out")
+    gate_p, gate_token, gate_head = (_heads(gate, shape, dt, "gate", device)
+                                     if gate is not None else (0, 0, 0))
+    table_p, n_seq, width = _table(table, None, device)
     ws, ws_bytes = 0, 0
     if workspace is not None:
-        if workspace.device != device or not workspace.is_contiguous():
-            raise ValueError(f"workspace: must be contiguous and on {device}")
+        if workspace.get_device() != device or not workspace.is_contiguous():
+            raise ValueError(f"workspace: must be contiguous and on cuda:{device}")
         ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    cu_q, seq_kv = _i32(cu_q, (n_seq + 1,), "cu_q", device), _i32(seq_kv, (n_seq,), "seq_kv", device)
-    table_p = _i32(table, (n_seq, None), "table", device)
-    if shape[0] == 0:
+    cu_p, kv_p = _i32(cu_q, n_seq + 1, "cu_q", device), _i32(seq_kv, n_seq, "seq_kv", device)
+    n_tok, h_q, _ = shape
+    if n_tok == 0:
         return 0
-    rows = ATTN_STRUCT.pack(
-        q_at[0], gate_at[0], out_at[0], cu_q, seq_kv, table_p, ws, ws_bytes, *q_at[1:],
-        *gate_at[1:], *out_at[1:], scale, shape[0], n_seq, shape[1], table.shape[1], max_q)
-    return _call("khq_paged_attn", rows, pages, stream_handle(stream), check=check)
+    rows = ATTN_STRUCT.pack(q_p, gate_p, out_p, cu_p, kv_p, table_p, ws, ws_bytes, q_token, q_head,
+                            gate_token, gate_head, out_token, out_head, scale, n_tok, n_seq, h_q,
+                            width, max_q)
+    return _call("khq_paged_attn", rows, pages, _stream(stream, device), check=check)
 
 
 def attn_ws_bytes(n_tok: int, n_seq: int, H_q: int, H_kv: int, head_dim: int, max_q: int) -> int:

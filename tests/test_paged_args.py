@@ -135,7 +135,7 @@ def test_overlapping_outputs_refused():
     for t in (x[:, None].expand(4, 3, 64), x[None].expand(2, 4, 64),
               x.as_strided((3, 2, 64), (32, 64, 1))):
         with pytest.raises(ValueError, match="overlap"):
-            paged._written(t, "out")
+            paged._written((0, *t.stride()[:2]), t.shape, "out")
     for t in (torch.zeros(4, 3, 64), torch.zeros(3, 4, 64).transpose(0, 1), torch.zeros(1, 1, 64),
               torch.zeros(4, 3, 128)[..., :64], torch.zeros(0, 3, 64)):
-        paged._written(t, "out")
+        paged._written((0, *t.stride()[:2]), t.shape, "out")
