@@ -46,7 +46,7 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t most, uint32
     return v;
 }
 
-// First index in [0, n) whose s[i + 1] > x (s increasing, s[n] > x).
+// First index in [0, n) whose s[i + 1] > x, s increasing (the last if none; s[n] is not read).
 __device__ __forceinline__ int find(const int* s, int n, int x) {
     int lo = 0, hi = n - 1;
     while (lo < hi) {
@@ -146,8 +146,8 @@ __global__ __launch_bounds__(PLAN_THR) void plan_kernel(PlanArgs a, int per, int
     extern __shared__ int s_mem[];
     __shared__ PlanLds lds;
     int* s_cu = s_mem;                // first rows, [n_seq + 1]
-    int* s_back = s_cu + a.n_seq + 1;  // pages given back before a request's, [n_seq + 1]
-    int* s_pre = s_back + a.n_seq + 1;  // new pages before a request's, -1: no slots
+    int* s_back = s_cu + a.n_seq + 1;  // pages given back before a request's
+    int* s_pre = s_back + a.n_seq;     // new pages before a request's, -1: no slots
     int* s_kv = s_pre + a.n_seq;
     Sums s;
     plan_sums(a, per, s, lds);
@@ -168,22 +168,15 @@ __global__ __launch_bounds__(PLAN_THR) void plan_kernel(PlanArgs a, int per, int
         }
     }
     __syncthreads();
-    if (blockIdx.x == 0) {
-        if (tid == 0) {
-            a.cu_q[0] = 0;
-            a.status[0] = lds.refused;
-            s_back[a.n_seq] = lds.n_back;
-        }
-        if (lds.n_back > 0) {
-            // ended requests' pages behind the free ones (entries that no new page is read from)
-            __syncthreads();
-            const int n_back = min(lds.n_back, a.n_pages - s.count);
-            for (int j = tid; j < n_back; j += thr) {
-                const int sq = find(s_back, a.n_seq, j);
-                a.free_pages[ring(a, s.head, s.count + j)] =
-                    a.table[(size_t)sq * a.table_ld + (j - s_back[sq])];
-            }
-        }
+    if (blockIdx.x == 0 && tid == 0) {
+        a.cu_q[0] = 0;
+        a.status[0] = lds.refused;
+    }
+    // ended requests' pages behind the free ones (entries that no new page is read from)
+    const int n_back = min(lds.n_back, a.n_pages - s.count);
+    for (int j = blockIdx.x * thr + tid; j < n_back; j += gridDim.x * thr) {
+        const int sq = find(s_back, a.n_seq, j);
+        a.free_pages[ring(a, s.head, s.count + j)] = a.table[(size_t)sq * a.table_ld + (j - s_back[sq])];
     }
     const int n_rows = s_cu[a.n_seq];
     const int t_end = min(a.n_tok, (int)(blockIdx.x + 1) * tok_per_block);
@@ -343,7 +336,7 @@ hipError_t launch_plan(const PlanArgs& a, bool in_place, hipStream_t st) {
     const int want = std::max(a.n_seq, std::min(a.n_tok, tok));
     const int thr = std::min(PLAN_THR, (want + 63) / 64 * 64);
     const bool later = in_place && blocks > 1;
-    const size_t lds = (4 * (size_t)a.n_seq + 2) * sizeof(int);
+    const size_t lds = (4 * (size_t)a.n_seq + 1) * sizeof(int);
     const hipError_t e = lds > 32768 ? ensure_dynamic_lds(reinterpret_cast<const void*>(plan_kernel), 66000)
                                      : hipSuccess;
     if (e != hipSuccess) return e;

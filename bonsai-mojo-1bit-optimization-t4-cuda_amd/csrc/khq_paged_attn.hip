@@ -13,6 +13,7 @@
 // step's 6 of 24 / 4 heads) stream keys and values through registers
 // (attn_stream_kernel), more go in tiles of 128 or 256 rows that share keys
 // and values in LDS (attn_tile_kernel).
+#include "khq_mfma_util.h"
 #include "khq_paged_internal.h"
 
 #include <algorithm>
@@ -94,7 +95,8 @@ constexpr float GAP = 10.0f * LOG2E;
 // Scores in log2 units, so that a weight is one exp2; not 0, whose product
 // with a masked score would be no number.
 __device__ __forceinline__ float score_scale(float scale) {
-    return fmaxf(fabsf(scale) * LOG2E, 1e-30f);
+    const float s = fmaxf(fabsf(scale) * LOG2E, 1e-30f);
+    return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(s)));  // a scalar register's
 }
 
 // ------------------------------------------------------------ the partition
@@ -113,13 +115,12 @@ struct Part {
     int unit;   // keys
     int slots;  // blocks
     Serve serve;
-    bool split;  // whether keys may be split
 };
 
 struct Item {
     int seq, row0, n_q, kv;  // sequence, its first batch row, rows and tokens
     int head, qt, split, n_split;
-    int block;  // of split 0; split i is block + i * H_kv
+    int part;  // partial result of split 0 where there are several; of split i: part + i * H_kv
 };
 
 struct SeqLen {
@@ -150,9 +151,13 @@ __device__ __forceinline__ T wave_sum(T v) {
 // Item x of the launch (joining: of those that are split).  Items are numbered
 // sequence by sequence; within one, KV heads in turn (blocks go to the XCDs in
 // turn, so a head's row tiles meet its keys in one L2), then splits, then row
-// tiles from the last, which sees most keys, to the first.  With items fewer
-// than slots the keys are split by the unit count u = cost / (slots - items):
-// sum of ceil(units / u) <= cost / u + items <= slots.
+// tiles from the last, which sees most keys, to the first.  A block takes at
+// most u units.  With items fewer than half the slots u = cost / (slots -
+// items): sum of ceil(units / u) <= cost / u + items <= slots, one round of
+// blocks.  With more, twice a slot's share of the cost, and from the slots' own
+// number on once that share: alike items stay whole, one of a long sequence
+// among short ones does not outlast the others.  Partial results: at most
+// 2 cost / u <= 2 slots, as an item that is split has more than u units.
 __device__ __forceinline__ bool schedule(const AttnArgs& a, const Part& pt, int x, bool joining,
                                          Item& it) {
     const int lane = threadIdx.x & 63, n_seq = a.r.n_seq, h_kv = a.p.H_kv;
@@ -165,37 +170,31 @@ __device__ __forceinline__ bool schedule(const AttnArgs& a, const Part& pt, int 
         items += one.tiles * h_kv;
         cost += (long long)one.tiles * h_kv * one.units;
     }
-    int u = 0x7fffffff;
-    if (pt.split) {
-        const int all = wave_sum(items);
-        if (all < pt.slots) {
-            const int room = pt.slots - all;
-            u = (int)min((wave_sum(cost) + room - 1) / room, 0x7fffffffll);
-            u = max(u, 1);
-        }
-    }
+    const int all = wave_sum(items);
+    const int room = all >= pt.slots ? pt.slots : max(pt.slots - all, pt.slots / 2);
+    const int u = (int)max(1ll, min((wave_sum(cost) + room - 1) / room, 0x7fffffffll));
     auto splits = [&](const SeqLen& l) { return (int)(((long long)l.units + u - 1) / u); };
-    int blocks = 0, found = 0;  // of this lane's sequences
+    int parts = 0, found = 0;  // of this lane's sequences
     for (int s = s0; s < s1; s++) {
         if (per > 1) one = seq_len(a, pt, s);
         const int n = one.tiles * h_kv, sp = splits(one);
-        blocks += n * sp;
+        parts += sp > 1 ? n * sp : 0;
         found += joining ? (sp > 1 ? n : 0) : n * sp;
     }
-    int upto = found, upto_b = blocks;
+    int upto = found, upto_p = parts;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(upto, o, 64), z = __shfl_up(upto_b, o, 64);
+        const int y = __shfl_up(upto, o, 64), z = __shfl_up(upto_p, o, 64);
         if (lane >= o) {
             upto += y;
-            upto_b += z;
+            upto_p += z;
         }
     }
     const unsigned long long past = __ballot(upto > x);
     if (past == 0) return false;
     const int owner = __ffsll(past) - 1;
     // the owner walks its sequences
-    int at = upto - found, block = upto_b - blocks, seq = s0;
+    int at = upto - found, part = upto_p - parts, seq = s0;
     if (lane == owner) {
         for (int s = s0; s < s1; s++) {
             if (per > 1) one = seq_len(a, pt, s);
@@ -204,7 +203,7 @@ __device__ __forceinline__ bool schedule(const AttnArgs& a, const Part& pt, int 
             const int c = joining ? (sp > 1 ? n : 0) : n * sp;
             if (x < at + c) break;
             at += c;
-            block += n * sp;
+            part += sp > 1 ? n * sp : 0;
         }
     }
     auto from = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
@@ -214,13 +213,12 @@ __device__ __forceinline__ bool schedule(const AttnArgs& a, const Part& pt, int 
     it.kv = from(one.kv);
     it.n_split = from(splits(one));
     const int tiles = from(one.tiles), j = x - from(at);
-    it.block = from(block);
     it.head = j % h_kv;
     const int k = j / h_kv;
     it.split = joining ? 0 : k % it.n_split;
     const int q = joining ? k : k / it.n_split;  // row tiles from the last
     it.qt = tiles - 1 - q;
-    it.block += q * it.n_split * h_kv + it.head;
+    it.part = from(part) + q * it.n_split * h_kv + it.head;
     return true;
 }
 
@@ -238,13 +236,13 @@ __device__ __forceinline__ long long token_at(const AttnArgs& a, const Item& it,
     return e * a.p.page_stride + in * a.p.token_stride + it.head * a.p.head_stride;
 }
 
-// Partial results: f32 [block][rows][D] (each kernel's own order of a block's
-// values), then (maximum, sum) f32 pairs [block][rows].
-__device__ __forceinline__ float* part_acc(float* ws, const Part& pt, int d, int block) {
-    return ws + (size_t)block * pt.rows * d;
+// Partial results: f32 [2 slots][rows][D] (each kernel's own order of one's
+// values), then (maximum, sum) f32 pairs [2 slots][rows].
+__device__ __forceinline__ float* part_acc(float* ws, const Part& pt, int d, int part) {
+    return ws + (size_t)part * pt.rows * d;
 }
-__device__ __forceinline__ float2* part_ml(float* ws, const Part& pt, int d, int block) {
-    return reinterpret_cast<float2*>(ws + (size_t)pt.slots * pt.rows * d) + (size_t)block * pt.rows;
+__device__ __forceinline__ float2* part_ml(float* ws, const Part& pt, int d, int part) {
+    return reinterpret_cast<float2*>(ws + (size_t)2 * pt.slots * pt.rows * d) + (size_t)part * pt.rows;
 }
 
 // ------------------------------------------------------------ few rows
@@ -442,7 +440,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
     __syncthreads();
     float* ws = static_cast<float*>(a.r.ws);
     const bool direct = it.n_split == 1;
-    const int block = it.block + it.split * a.p.H_kv;
+    const int part = it.part + it.split * a.p.H_kv;
     for (int i = tid; i < rows * (D / 4); i += 64 * NW) {
         const int row = i / (D / 4), c = (i % (D / 4)) * 4;
         float m = s_m[0][row];
@@ -470,8 +468,8 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
             *reinterpret_cast<u2e*>((T*)a.r.out + (it.row0 + tok) * a.r.out_token + hq * a.r.out_head + c) =
                 u2e{pack<T>(o[0], o[1]), pack<T>(o[2], o[3])};
         } else {
-            *reinterpret_cast<f4*>(part_acc(ws, pt, D, block) + row * D + c) = o;
-            if (c == 0) part_ml(ws, pt, D, block)[row] = float2{m, l};
+            *reinterpret_cast<f4*>(part_acc(ws, pt, D, part) + row * D + c) = o;
+            if (c == 0) part_ml(ws, pt, D, part)[row] = float2{m, l};
         }
     }
 }
@@ -481,40 +479,59 @@ template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void attn_stream_join_kernel(AttnArgs a, Part pt) {
     constexpr int E = D / 64, RB = 4 / W;  // dims a lane, rows a block
     typedef float fe __attribute__((ext_vector_type(E)));
-    __shared__ float s_o[W > 1 ? W : 1][D], s_l[4];
+    __shared__ float s_o[W > 1 ? W : 1][D];
+    __shared__ float2 s_ml[W];
     Item it;
     if (!schedule(a, pt, blockIdx.x / (16 / RB), true, it)) return;
     const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, h_kv = a.p.H_kv;
     const int row = blockIdx.x % (16 / RB) * RB + wv / W, r = it.qt * 16 + row;
     if (r >= it.n_q * a.n_rep) return;  // (W > 1: of the whole block)
     float* ws = static_cast<float*>(a.r.ws);
-    float m = M_NONE;
-    for (int i = lane; i < it.n_split; i += 64)
-        m = fmaxf(m, part_ml(ws, pt, D, it.block + i * h_kv)[row].x);
-#pragma unroll
-    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    const int tok = a.by_rep.div(r), hq = it.head * a.n_rep + r - tok * a.n_rep;
     fe o = {};
-    float l = 0.0f;
-#pragma unroll 8
-    for (int i = wv % W; i < it.n_split; i += W) {
-        const float2 ml = part_ml(ws, pt, D, it.block + i * h_kv)[row];
-        const fe x = *reinterpret_cast<const fe*>(part_acc(ws, pt, D, it.block + i * h_kv) + row * D + E * lane);
-        const float f = __builtin_amdgcn_exp2f(ml.x - m);
-        l += ml.y * f;
-        o += x * f;
+    float m = M_NONE, l = 0.0f;
+    // eight splits in flight, their maxima with them
+    for (int i0 = wv % W; i0 < it.n_split; i0 += 8 * W) {
+        float2 ml[8];
+        fe x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int i = min(i0 + j * W, it.n_split - 1);
+            ml[j] = part_ml(ws, pt, D, it.part + i * h_kv)[row];
+            x[j] = *reinterpret_cast<const fe*>(part_acc(ws, pt, D, it.part + i * h_kv) + row * D + E * lane);
+        }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = fmaxf(top, ml[j].x);
+        const float f0 = __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l *= f0;
+        o *= f0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (i0 + j * W >= it.n_split) break;
+            const float f = __builtin_amdgcn_exp2f(ml[j].x - m);
+            l += ml[j].y * f;
+            o += x[j] * f;
+        }
     }
     if constexpr (W > 1) {
 #pragma unroll
         for (int e = 0; e < E; e++) s_o[wv][E * lane + e] = o[e];
-        if (lane == 0) s_l[wv] = l;
+        if (lane == 0) s_ml[wv] = float2{m, l};
         __syncthreads();
         if (wv > 0) return;
-        l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+        m = fmaxf(fmaxf(s_ml[0].x, s_ml[1].x), fmaxf(s_ml[2].x, s_ml[3].x));
+        l = 0.0f;
+        o = fe{};
 #pragma unroll
-        for (int e = 0; e < E; e++)
-            o[e] = (s_o[0][E * lane + e] + s_o[1][E * lane + e]) + (s_o[2][E * lane + e] + s_o[3][E * lane + e]);
+        for (int w = 0; w < W; w++) {
+            const float f = __builtin_amdgcn_exp2f(s_ml[w].x - m);
+            l += s_ml[w].y * f;
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] += s_o[w][E * lane + e] * f;
+        }
     }
-    const int tok = a.by_rep.div(r), hq = it.head * a.n_rep + r - tok * a.n_rep;
     const float inv = visible(a, it, r) > 0 ? 1.0f / l : 0.0f;
     const T* gate = (const T*)a.r.gate + (it.row0 + tok) * a.r.gate_token + hq * a.r.gate_head + E * lane;
     T* out = (T*)a.r.out + (it.row0 + tok) * a.r.out_token + hq * a.r.out_head + E * lane;
@@ -534,6 +551,16 @@ __device__ __forceinline__ void load_lds16(const void* g, uint32_t to) {
                  "s"(__builtin_amdgcn_readfirstlane(to))
                  : "memory");
 }
+__device__ __forceinline__ long long uniform(long long x) {
+    const int lo = __builtin_amdgcn_readfirstlane((int)x), hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
+    return ((long long)hi << 32) | (uint32_t)lo;
+}
+// The same from a uniform address and a lane's bytes.
+__device__ __forceinline__ void load_lds16(const void* g, uint32_t bytes, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(bytes), "s"(g),
+                 "s"(__builtin_amdgcn_readfirstlane(to))
+                 : "memory");
+}
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // Four keys' values of a lane's dim: each 16 lanes read a 4 x 16 block whose
 // row j lies at lanes 4 j .. 4 j + 3, and lane i gets its column i.
@@ -543,7 +570,20 @@ __device__ __forceinline__ u2 read_tr(const char* p) {
                                       (__attribute__((address_space(3))) s4*)p));
 }
 
-constexpr int TAB = 2048;  // block table entries in LDS
+constexpr int TAB = 1024;  // pages whose byte offsets are in LDS (-1: not a page)
+
+// x, of which the compiler knows nothing: what follows from it is computed where
+// it is used, and not kept in registers that there are not.
+__device__ __forceinline__ int opaque(int x) {
+    asm("" : "+v"(x));
+    return x;
+}
+// The lane, without a register that holds it until then.
+__device__ __forceinline__ int lane_again() {
+    int l;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+    return l;
+}
 
 // Row r of the item: its output, times the gate, four dims from dim on.
 template <typename T>
@@ -574,14 +614,18 @@ template <typename T, int D, int KG>
 __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) {
     constexpr int NS = D / 16, ND = D / 32;  // K steps of a score, dim tiles
     constexpr int ROW = 2 * D, SLOT = 64 * ROW;  // bytes
-    constexpr int CH = D / 8, KPI = 64 / CH, NI = 64 / KPI / 8;  // pieces a row, keys a load, loads
+    constexpr int CH = D / 8, KPI = 64 / CH, NL = 16 / KPI;  // pieces a row, keys a load, loads of 16 keys
+    constexpr int AHEAD = D == 64 ? 4 : D == 128 ? 6 : 3;
+    // Q operands that stay in LDS: a register file holds 128 of O, 64 of Q, 16
+    // scores and 16 of operands, and a few too few for what goes with them.
+    constexpr int QL = D == 256 ? 2 : 0;
     typedef typename V<T>::x8 x8;
     extern __shared__ __align__(1024) char lds[];
     char* const ks = lds;
     char* const vs = lds + 2 * SLOT;
-    int* const tab = reinterpret_cast<int*>(lds + 4 * SLOT);
+    long long* const tab = reinterpret_cast<long long*>(lds + 4 * SLOT);
     __shared__ int s_bad;
-    __shared__ float s_m[4][32], s_l[4][32];
+    __shared__ float2 s_ml[2][4][32];
     Item it;
     if (!schedule(a, pt, blockIdx.x, false, it)) return;
     const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -589,50 +633,76 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
     const int rg = KG == 1 ? wv : wv & 3, kg = KG == 1 ? 0 : wv >> 2;
     constexpr int BR = 256 / KG;
     const int n_rows = it.n_q * a.n_rep;
-    const int r = it.qt * BR + rg * 32 + ln;
-    const bool r_ok = r < n_rows;
-    // (a lane of no row sees what the last row sees and stores nothing)
-    const int vis = visible(a, it, min(r, n_rows - 1));
+    // (a lane of no row is the last row again and stores nothing)
+    const int r_in = min(it.qt * BR + rg * 32 + ln, n_rows - 1);
+    const int vis = visible(a, it, r_in);
     const int vis_hi = visible(a, it, min(it.qt * BR + BR, n_rows) - 1);
     const int units = (vis_hi + 63) >> 6;
     const int u_lo = (int)((long long)units * it.split / it.n_split);
     const int u_hi = (int)((long long)units * (it.split + 1) / it.n_split);
-    x8 qb[NS];
+    x8 qb[NS - QL];
+    char* const ql = lds + 4 * SLOT + TAB * (int)sizeof(long long) + wv * (QL * 1024) + lane * 16;
     {
         const uint32_t flip = a.r.scale < 0.0f ? 0x80008000u : 0u;
-        const int rr = min(r, n_rows - 1), tok = a.by_rep.div(rr);
+        const int tok = a.by_rep.div(r_in);
         const T* q = (const T*)a.r.q + (it.row0 + tok) * a.r.q_token +
-                     (it.head * a.n_rep + rr - tok * a.n_rep) * a.r.q_head + 8 * hh;
+                     (it.head * a.n_rep + r_in - tok * a.n_rep) * a.r.q_head + 8 * hh;
 #pragma unroll
         for (int st = 0; st < NS; st++) {
             const u4e v = *reinterpret_cast<const u4e*>(q + 16 * st);
-            qb[st] = __builtin_bit_cast(x8, u4{v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip});
+            const u4 w = {v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip};
+            if (st < QL) *reinterpret_cast<u4*>(ql + st * 1024) = w;
+            else qb[st - QL] = __builtin_bit_cast(x8, w);
         }
     }
+    const int q_at = lds_addr(ql) - lds_addr(lds);
     const float sc2 = score_scale(a.r.scale);
     int w0 = 0;  // first page of the table's window
-    auto fill = [&](int u) {
+    auto fill = [&](int u) __attribute__((always_inline)) {
         w0 = a.by_page.div(u * 64);
         const int n = min(TAB, a.by_page.div(vis_hi - 1) + 1 - w0);
-        for (int i = tid; i < n; i += 512) {
+        for (int i = wv * 64 + lane_again(); i < n; i += 512) {
             const int e = a.r.table[(size_t)it.seq * a.r.table_ld + w0 + i];
             const bool bad = (unsigned)e >= (unsigned)a.p.n_pages;
-            tab[i] = bad ? -1 : e;
+            tab[i] = bad ? -1 : 2 * (e * a.p.page_stride);
             if (bad) s_bad = 1;
         }
     };
-    auto stage = [&](int u, int slot) {
+    // A unit into a slot, by wavefronts 4 to 7: 16 keys each, NL loads of 1 KB of
+    // K and of V.  A load takes the address unit 16 cycles, and a wavefront
+    // waits where others' are before its own: while these four do, the other
+    // wavefront of each SIMD has the matrix cores, and they have them while it
+    // takes its weights.  Where the 16 keys lie in one page, as they do in pages
+    // of a multiple of 16, an address is a scalar and a lane's constant; else
+    // each lane looks its key up.
+    const char* const kh = (const char*)a.p.k + 2 * (it.head * a.p.head_stride);
+    const char* const vh = (const char*)a.p.v + 2 * (it.head * a.p.head_stride);
+    const int last = vis_hi - 1;
+    const bool by_group = a.p.page_size % 16 == 0 && a.p.token_stride * a.p.page_size < 1 << 28;
+    auto stage = [&](int u) __attribute__((always_inline)) {
+        const int w = wv & 3, l = lane_again(), lk = l / CH, p = l % CH;
+        const uint32_t to = ((u - u_lo) & 1) * SLOT + w * NL * 1024;
+        auto piece_k = [&](int key) { return (p ^ (D == 64 ? (key >> 1) & 7 : key & 15)) << 4; };
+        auto piece_v = [&](int key) { return (p ^ (D == 64 ? (key & 2) << 1 : (key & 3) << 2)) << 4; };
+        if (by_group) {
+            const int t = min(u * 64 + w * 16, last & ~15), pg = a.by_page.div(t);
+            const int ts2 = 2 * (int)a.p.token_stride;
+            const long long at = uniform(max(uniform(tab[pg - w0]), 0ll) + (t - pg * a.p.page_size) * ts2);
+            const int most = last - t;
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const int key = (wv * NI + i) * KPI + lane / CH, p = lane % CH;
-            const int t = min(u * 64 + key, vis_hi - 1);
-            const int pg = a.by_page.div(t);
-            const long long off = max(tab[pg - w0], 0) * a.p.page_stride +
-                                  (t - pg * a.p.page_size) * a.p.token_stride + it.head * a.p.head_stride;
-            const int fk = D == 64 ? (key >> 1) & 7 : key & 15;
-            const int fv = D == 64 ? (key & 2) << 1 : (key & 3) << 2;
-            load_lds16((const T*)a.p.k + off + 8 * (p ^ fk), lds_addr(ks) + slot * SLOT + (wv * NI + i) * 1024);
-            load_lds16((const T*)a.p.v + off + 8 * (p ^ fv), lds_addr(vs) + slot * SLOT + (wv * NI + i) * 1024);
+            for (int i = 0; i < NL; i++) {
+                const int row = i * KPI + lk, key = w * 16 + row, off = min(row, most) * ts2;
+                load_lds16(kh + at, off + piece_k(key), lds_addr(ks) + to + i * 1024);
+                load_lds16(vh + at, off + piece_v(key), lds_addr(vs) + to + i * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int key = w * 16 + i * KPI + lk, t = min(u * 64 + key, last), pg = a.by_page.div(t);
+                const long long off = max(tab[pg - w0], 0ll) + 2 * ((t - pg * a.p.page_size) * a.p.token_stride);
+                load_lds16(kh + off + piece_k(key), lds_addr(ks) + to + i * 1024);
+                load_lds16(vh + off + piece_v(key), lds_addr(vs) + to + i * 1024);
+            }
         }
     };
     f16v acc[ND];
@@ -651,10 +721,10 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
     if (u_lo < u_hi) {
         fill(u_lo);
         __syncthreads();
-        stage(u_lo, 0);
+        if (wv >= 4) stage(u_lo);
     }
     // unit u is waited for, the next one started
-    auto begin = [&](int u) {
+    auto begin = [&](int u) __attribute__((always_inline)) {
         wait_loads();
         __syncthreads();  // u is there, u - 1 is done with
         if (u + 1 < u_hi) {
@@ -662,10 +732,10 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
                 fill(u);
                 __syncthreads();
             }
-            stage(u + 1, (u + 1 - u_lo) & 1);
+            if (wv >= 4) stage(u + 1);
         }
     };
-    auto keys = [&](int u, auto masked) {
+    auto keys = [&](int u, auto masked) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
 #pragma unroll 1
         for (int sub = kg; sub < 2; sub += KG) {
@@ -674,19 +744,32 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
             const int at = ((u - u_lo) & 1) * SLOT + sub * 32 * ROW;
             const char* const kb = ks + at;
             const char* const vb = vs + at;
-            // (opaque: the permuted places are a xor each, and would be kept in
-            // registers that there are not)
-            int ka = k_at, va = v_at;
-            asm("" : "+v"(ka), "+v"(va));
-            f16v s2[2];
+            const int ka = opaque(k_at), va = opaque(v_at);  // (the permuted places: a xor each)
+            // An operand's read is AHEAD products before its own.
+            x8 kf[AHEAD + 1];
+            auto read_k = [&](int st) {
+                kf[st % (AHEAD + 1)] = *reinterpret_cast<const x8*>(kb + (ka ^ (st << 5)));
+            };
+            u4 vf[AHEAD + 1];  // dim tile n / 2, K step n % 2
+            auto read_v = [&](int n) {
+                const char* const p = vb + (va ^ ((n >> 1) << 6)) + 16 * (n & 1) * ROW;
+                const u2 lo = read_tr(p), hi = read_tr(p + 8 * ROW);
+                vf[n % (AHEAD + 1)] = u4{lo.x, lo.y, hi.x, hi.y};
+            };
+            f16v sc;
 #pragma unroll
-            for (int e = 0; e < 16; e++) s2[0][e] = s2[1][e] = 0.0f;
+            for (int e = 0; e < 16; e++) sc[e] = 0.0f;
 #pragma unroll
-            for (int st = 0; st < NS; st++)
-                s2[st & 1] = mfma32(*reinterpret_cast<const x8*>(kb + (ka ^ (st << 5))), qb[st], s2[st & 1]);
-            float sc[16];
+            for (int st = 0; st < AHEAD; st++) read_k(st);
 #pragma unroll
-            for (int e = 0; e < 16; e++) sc[e] = s2[0][e] + s2[1][e];
+            for (int st = 0; st < NS; st++) {
+                if (st + AHEAD < NS) read_k(st + AHEAD);
+                else read_v(st + AHEAD - NS);
+                __builtin_amdgcn_sched_barrier(0);
+                sc = mfma32(kf[st % (AHEAD + 1)],
+                            st < QL ? *reinterpret_cast<const x8*>(lds + q_at + st * 1024) : qb[max(st - QL, 0)], sc);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             bool odd = false;  // values that are no numbers where a row's mask has to hold
             if constexpr (MASKED) {
                 if (s_bad) {
@@ -752,17 +835,15 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
                 }
             }
 #pragma unroll
-            for (int i = 0; i < ND; i++)
-#pragma unroll
-                for (int sp = 0; sp < 2; sp++) {
-                    const char* const p = vb + (va ^ (i << 6)) + 16 * sp * ROW;
-                    u2 lo = read_tr(p), hi = read_tr(p + 8 * ROW);
-                    if (MASKED && odd) {  // ... and leave the product
-                        lo = u2{finite_pair<T>(lo.x), finite_pair<T>(lo.y)};
-                        hi = u2{finite_pair<T>(hi.x), finite_pair<T>(hi.y)};
-                    }
-                    acc[i] = mfma32(__builtin_bit_cast(x8, u4{lo.x, lo.y, hi.x, hi.y}), pb[sp], acc[i]);
-                }
+            for (int n = 0; n < 2 * ND; n++) {
+                if (n + AHEAD < 2 * ND) read_v(n + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+                u4 v = vf[n % (AHEAD + 1)];
+                if (MASKED && odd)  // ... and leave the product
+                    v = u4{finite_pair<T>(v.x), finite_pair<T>(v.y), finite_pair<T>(v.z), finite_pair<T>(v.w)};
+                acc[n >> 1] = mfma32(__builtin_bit_cast(x8, v), pb[n & 1], acc[n >> 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
     // units that every row sees whole, then the others; all from the first entry
@@ -781,88 +862,153 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
         keys(u, std::true_type{});
     }
     float l_row = l_part + __shfl_xor(l_part, 32, 64);
-    if constexpr (KG == 2) {  // the other half of the keys
-        __syncthreads();
-        f4* const x = reinterpret_cast<f4*>(lds) + rg * (ND * 4 * 64) + lane;
-        if (kg == 1) {
+    __syncthreads();  // the slots are free: 32 rows of half the dims for each wavefront
+    constexpr int HD = ND / 2, AREA = 32 * (D / 2) * (int)sizeof(float);
+    const int el = lane_again(), eln = el & 31, ehh = el >> 5;
+    // ---- dims dim0 + 32 i + 8 q + 4 ehh + c of row eln leave
+    auto leave = [&](const f16v(&res)[HD], int half, char* area) __attribute__((always_inline)) {
+        const int r0 = it.qt * BR + rg * 32;
+        if (it.n_split > 1) {
+            float* ws = static_cast<float*>(a.r.ws);
+            const int part = it.part + it.split * a.p.H_kv;
+            f4* const x = reinterpret_cast<f4*>(part_acc(ws, pt, D, part)) + (rg * ND + half * HD) * (4 * 64) + el;
 #pragma unroll
-            for (int i = 0; i < ND; i++)
+            for (int i = 0; i < HD; i++)
 #pragma unroll
                 for (int q = 0; q < 4; q++)
-                    x[(i * 4 + q) * 64] = f4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
-            if (hh == 0) {
-                s_m[rg][ln] = m_ref;
-                s_l[rg][ln] = l_row;
-            }
+                    x[(i * 4 + q) * 64] = f4{res[i][4 * q], res[i][4 * q + 1], res[i][4 * q + 2], res[i][4 * q + 3]};
+            if (ehh == 0 && half == 0) part_ml(ws, pt, D, part)[rg * 32 + eln] = float2{m_ref, l_row};
+            return;
         }
-        __syncthreads();
-        if (kg == 1) return;
-        const float m2 = s_m[rg][ln], m = fmaxf(m_ref, m2);
-        const float f1 = __builtin_amdgcn_exp2f(m_ref - m), f2 = __builtin_amdgcn_exp2f(m2 - m);
-        m_ref = m;
-        l_row = l_row * f1 + s_l[rg][ln] * f2;
+        // through LDS, so that a lane stores 16 bytes next to its neighbours'
+        constexpr int CN = D / 8, GN = D / 16, RI = 64 / GN;  // pieces and 8-dim groups of a half row, rows at once
+        const float inv = vis > 0 ? 1.0f / l_row : 0.0f;
+        mu::wave_sync();
 #pragma unroll
-        for (int i = 0; i < ND; i++)
+        for (int i = 0; i < HD; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                *reinterpret_cast<f4*>(area + eln * (CN * 16) + (((8 * i + 2 * q + ehh) ^ (eln & (CN - 1))) << 4)) =
+                    f4{res[i][4 * q], res[i][4 * q + 1], res[i][4 * q + 2], res[i][4 * q + 3]} * inv;
+        mu::wave_sync();
+        const int g = el % GN, dim = half * (D / 2) + 8 * g;
+        u4 gate[32 / RI];
+        T* out[32 / RI];
+#pragma unroll
+        for (int k = 0; k < 32 / RI; k++) {
+            const int r = r0 + k * RI + el / GN, rr = min(r, n_rows - 1), tok = a.by_rep.div(rr);
+            const int hq = it.head * a.n_rep + rr - tok * a.n_rep;
+            out[k] = r < n_rows ? (T*)a.r.out + (it.row0 + tok) * a.r.out_token + hq * a.r.out_head + dim : nullptr;
+            gate[k] = u4{0u, 0u, 0u, 0u};
+            if (a.r.gate)
+                gate[k] = *reinterpret_cast<const u4e*>((const T*)a.r.gate + (it.row0 + tok) * a.r.gate_token +
+                                                        hq * a.r.gate_head + dim);
+        }
+#pragma unroll
+        for (int k = 0; k < 32 / RI; k++) {
+            const int row = k * RI + el / GN, s = row & (CN - 1);
+            const f4 x = *reinterpret_cast<const f4*>(area + row * (CN * 16) + (((2 * g) ^ s) << 4));
+            const f4 y = *reinterpret_cast<const f4*>(area + row * (CN * 16) + (((2 * g + 1) ^ s) << 4));
+            float o[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            if (a.r.gate) {
+                const x8 gv = __builtin_bit_cast(x8, gate[k]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) o[e] *= sigmoid(gv[e]);
+            }
+            if (out[k])
+                *reinterpret_cast<u4e*>(out[k]) = u4e{pack<T>(o[0], o[1]), pack<T>(o[2], o[3]),
+                                                      pack<T>(o[4], o[5]), pack<T>(o[6], o[7])};
+        }
+    };
+    if constexpr (KG == 1) {
+        f16v res[HD];
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+#pragma unroll
+            for (int i = 0; i < HD; i++) res[i] = acc[half * HD + i];
+            leave(res, half, lds + wv * AREA);
+        }
+    } else {
+        // the two halves of a row's keys: wavefront kg joins and stores half kg of the dims
+        f16v res[HD];
+        auto give = [&](const f16v* from) {
+            f4* const x = reinterpret_cast<f4*>(lds + (rg * 2 + kg) * AREA) + el;
+#pragma unroll
+            for (int i = 0; i < HD; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    x[(i * 4 + q) * 64] = f4{from[i][4 * q], from[i][4 * q + 1], from[i][4 * q + 2], from[i][4 * q + 3]};
+        };
+        if (kg == 0) {
+            give(acc + HD);
+#pragma unroll
+            for (int i = 0; i < HD; i++) res[i] = acc[i];
+        } else {
+            give(acc);
+#pragma unroll
+            for (int i = 0; i < HD; i++) res[i] = acc[HD + i];
+        }
+        if (ehh == 0) s_ml[kg][rg][eln] = float2{m_ref, l_row};
+        __syncthreads();
+        const float2 ml = s_ml[1 - kg][rg][eln];
+        const float m = fmaxf(m_ref, ml.x);
+        const float f1 = __builtin_amdgcn_exp2f(m_ref - m), f2 = __builtin_amdgcn_exp2f(ml.x - m);
+        m_ref = m;
+        l_row = l_row * f1 + ml.y * f2;
+        char* const area = lds + (rg * 2 + 1 - kg) * AREA;
+        const f4* const x = reinterpret_cast<const f4*>(area) + el;
+#pragma unroll
+        for (int i = 0; i < HD; i++)
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 const f4 o = x[(i * 4 + q) * 64];
 #pragma unroll
-                for (int c = 0; c < 4; c++) acc[i][4 * q + c] = acc[i][4 * q + c] * f1 + o[c] * f2;
+                for (int c = 0; c < 4; c++) res[i][4 * q + c] = res[i][4 * q + c] * f1 + o[c] * f2;
             }
-    }
-    // ---- dims 32 i + 8 q + 4 hh + c of row r
-    if (it.n_split == 1) {
-        if (!r_ok) return;
-        const float inv = vis > 0 ? 1.0f / l_row : 0.0f;
-#pragma unroll
-        for (int i = 0; i < ND; i++)
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                store_row4<T>(a, it, r, 32 * i + 8 * q + 4 * hh,
-                              f4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]} * inv);
-    } else {
-        float* ws = static_cast<float*>(a.r.ws);
-        const int block = it.block + it.split * a.p.H_kv;
-        f4* const x = reinterpret_cast<f4*>(part_acc(ws, pt, D, block)) + rg * (ND * 4 * 64) + lane;
-#pragma unroll
-        for (int i = 0; i < ND; i++)
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                x[(i * 4 + q) * 64] = f4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
-        if (hh == 0) part_ml(ws, pt, D, block)[rg * 32 + ln] = float2{m_ref, l_row};
+        leave(res, kg, area);
     }
 }
 
-// The splits of 32 rows, a wavefront 32 dims of them.
+// The splits of 32 rows: a wavefront 8 dims of them, a block 32.
 template <typename T, int D>
-__global__ __launch_bounds__(2 * D) void attn_tile_join_kernel(AttnArgs a, Part pt) {
+__global__ __launch_bounds__(256) void attn_tile_join_kernel(AttnArgs a, Part pt) {
     constexpr int ND = D / 32;
     const int groups = pt.rows / 32;
     Item it;
-    if (!schedule(a, pt, blockIdx.x / groups, true, it)) return;
-    const int rg = blockIdx.x % groups;
-    const int i = threadIdx.x >> 6, lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5;
+    if (!schedule(a, pt, blockIdx.x / (groups * ND), true, it)) return;
+    const int rg = blockIdx.x / ND % groups, i = blockIdx.x % ND;
+    const int q = threadIdx.x >> 6, lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5;
     const int r = it.qt * pt.rows + rg * 32 + ln, h_kv = a.p.H_kv;
-    if (it.qt * pt.rows + rg * 32 >= it.n_q * a.n_rep) return;
-    float* ws = static_cast<float*>(a.r.ws);
-    float m = M_NONE, l = 0.0f;
-    for (int s = 0; s < it.n_split; s++)
-        m = fmaxf(m, part_ml(ws, pt, D, it.block + s * h_kv)[rg * 32 + ln].x);
-    f4 o[4] = {};
-#pragma unroll 4
-    for (int s = 0; s < it.n_split; s++) {
-        const float2 ml = part_ml(ws, pt, D, it.block + s * h_kv)[rg * 32 + ln];
-        const f4* x = reinterpret_cast<const f4*>(part_acc(ws, pt, D, it.block + s * h_kv)) +
-                      (rg * ND + i) * (4 * 64) + lane;
-        const float f = __builtin_amdgcn_exp2f(ml.x - m);
-        l += ml.y * f;
-#pragma unroll
-        for (int q = 0; q < 4; q++) o[q] += x[q * 64] * f;
-    }
     if (r >= it.n_q * a.n_rep) return;
-    const float inv = visible(a, it, r) > 0 ? 1.0f / l : 0.0f;
+    float* ws = static_cast<float*>(a.r.ws);
+    f4 o = {};
+    float m = M_NONE, l = 0.0f;
+    for (int s0 = 0; s0 < it.n_split; s0 += 8) {
+        float2 ml[8];
+        f4 x[8];
 #pragma unroll
-    for (int q = 0; q < 4; q++) store_row4<T>(a, it, r, 32 * i + 8 * q + 4 * hh, o[q] * inv);
+        for (int j = 0; j < 8; j++) {
+            const int s = min(s0 + j, it.n_split - 1);
+            ml[j] = part_ml(ws, pt, D, it.part + s * h_kv)[rg * 32 + ln];
+            x[j] = reinterpret_cast<const f4*>(part_acc(ws, pt, D, it.part + s * h_kv))[((rg * ND + i) * 4 + q) * 64 + lane];
+        }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = fmaxf(top, ml[j].x);
+        const float f0 = __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l *= f0;
+        o *= f0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (s0 + j >= it.n_split) break;
+            const float f = __builtin_amdgcn_exp2f(ml[j].x - m);
+            l += ml[j].y * f;
+            o += x[j] * f;
+        }
+    }
+    const float inv = visible(a, it, r) > 0 ? 1.0f / l : 0.0f;
+    store_row4<T>(a, it, r, 32 * i + 8 * q + 4 * hh, o * inv);
 }
 
 // What a call of these sizes launches.
@@ -871,38 +1017,42 @@ struct Plan {
     Part ps, pl;
     int stream_blocks, stream_joins, tile_blocks, tile_joins, kg;
 };
+// Blocks for up to `items` items: one round of slots while they may be few,
+// else cost / u more than items (schedule), u at least half a slot's share.
+int blocks_for(long long items, int slots) {
+    return (int)(items + slots);
+}
 Plan plan_of(int n_tok, int n_seq, int H_q, int H_kv, int max_q) {
     const int n_rep = H_q / H_kv, seqs = std::min(n_tok, n_seq);
     const long long rows = (long long)n_tok * n_rep;
     Plan p{};
     p.stream = true;  // there may be short sequences whatever max_q says
     p.tile = (long long)max_q * n_rep > SMALL_ROWS;
-    p.ps = Part{16, STREAM_UNIT, STREAM_SLOTS, p.tile ? SERVE_SMALL : SERVE_ALL, true};
+    p.ps = Part{16, STREAM_UNIT, STREAM_SLOTS, p.tile ? SERVE_SMALL : SERVE_ALL};
     // row tiles there may be: those served hold 16 rows or, served all, n_tok's
     const long long most = p.tile ? (long long)seqs * H_kv : (rows / 16 + seqs) * H_kv;
-    p.stream_blocks = (int)std::max<long long>(STREAM_SLOTS, most);
+    p.stream_blocks = blocks_for(most, STREAM_SLOTS);
     p.stream_joins = (int)std::min<long long>(STREAM_SLOTS, most);
     p.kg = rows / 256 * H_kv >= TILE_SLOTS ? 1 : 2;
     const int br = 256 / p.kg;
-    p.pl = Part{br, TILE_UNIT, TILE_SLOTS, SERVE_LARGE, rows / br * H_kv < TILE_SLOTS};
+    p.pl = Part{br, TILE_UNIT, TILE_SLOTS, SERVE_LARGE};
     const long long tiles = (rows / br + seqs) * H_kv;
-    p.tile_blocks = (int)std::max<long long>(p.pl.split ? TILE_SLOTS : 0, tiles);
+    p.tile_blocks = blocks_for(tiles, TILE_SLOTS);
     p.tile_joins = (int)std::min<long long>(TILE_SLOTS, tiles);
     return p;
 }
 size_t part_bytes(const Part& pt, int d) {
-    return pt.split ? (size_t)pt.slots * pt.rows * (d * sizeof(float) + sizeof(float2)) : 0;
+    return (size_t)2 * pt.slots * pt.rows * (d * sizeof(float) + sizeof(float2));
 }
 
 template <typename T, int D, int KG>
 hipError_t launch_tile(const AttnArgs& a, const Plan& p, hipStream_t st) {
-    constexpr int bytes = 4 * 64 * 2 * D + TAB * (int)sizeof(int);
+    constexpr int bytes = 4 * 64 * 2 * D + TAB * (int)sizeof(long long) + (D == 256 ? 8 * 2 * 1024 : 0);
     const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(attn_tile_kernel<T, D, KG>), bytes);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((attn_tile_kernel<T, D, KG>), dim3(p.tile_blocks), dim3(512), bytes, st, a, p.pl);
-    if (p.pl.split)
-        hipLaunchKernelGGL((attn_tile_join_kernel<T, D>), dim3(p.tile_joins * (p.pl.rows / 32)), dim3(2 * D),
-                           0, st, a, p.pl);
+    hipLaunchKernelGGL((attn_tile_join_kernel<T, D>), dim3(p.tile_joins * (p.pl.rows / 32) * (D / 32)),
+                       dim3(256), 0, st, a, p.pl);
     return hipGetLastError();
 }
 
