@@ -81,7 +81,7 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t p) {  // those as zeros
 }
 template <typename T>
 __device__ __forceinline__ float sigmoid(T g) {
-    return 1.0f / (1.0f + __expf(-(float)g));
+    return __builtin_amdgcn_rcpf(1.0f + __expf(-(float)g));  // each to a unit of 2^-23
 }
 
 // Reference maximum of a row that has seen no key: finite, so that a masked
@@ -141,65 +141,105 @@ __device__ __forceinline__ SeqLen seq_len(const AttnArgs& a, const Part& pt, int
     return l;
 }
 
+// Inclusive sums over the lanes: within rows of 16, then rows to the right of
+// lanes 15, 31 and 47.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_from(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int as_bits(int v) { return v; }
+__device__ __forceinline__ int as_bits(float v) { return __float_as_int(v); }
 template <typename T>
-__device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
+__device__ __forceinline__ T scan_add(T v) {
+    auto of = [](int x) { return __builtin_bit_cast(T, x); };
+    v += of(dpp_from<0x111, 0xF>(as_bits(v)));  // row_shr 1, 2, 4, 8
+    v += of(dpp_from<0x112, 0xF>(as_bits(v)));
+    v += of(dpp_from<0x114, 0xF>(as_bits(v)));
+    v += of(dpp_from<0x118, 0xF>(as_bits(v)));
+    v += of(dpp_from<0x142, 0xA>(as_bits(v)));  // row_bcast 15, 31
+    v += of(dpp_from<0x143, 0xC>(as_bits(v)));
     return v;
 }
+template <typename T>
+__device__ __forceinline__ T lane63(T v) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(as_bits(v), 63));
+}
 
-// Item x of the launch (joining: of those that are split).  Items are numbered
-// sequence by sequence; within one, KV heads in turn (blocks go to the XCDs in
-// turn, so a head's row tiles meet its keys in one L2), then splits, then row
-// tiles from the last, which sees most keys, to the first.  A block takes at
-// most u units.  With items fewer than half the slots u = cost / (slots -
-// items): sum of ceil(units / u) <= cost / u + items <= slots, one round of
-// blocks.  With more, twice a slot's share of the cost, and from the slots' own
-// number on once that share: alike items stay whole, one of a long sequence
-// among short ones does not outlast the others.  Partial results: at most
-// 2 cost / u <= 2 slots, as an item that is split has more than u units.
-__device__ __forceinline__ bool schedule(const AttnArgs& a, const Part& pt, int x, bool joining,
-                                         Item& it) {
+// The partition: items (row tile of a KV head) and what they are split into.
+// Items are numbered sequence by sequence, with LONG (and up to 64 sequences)
+// those of the longest blocks first; within a sequence, KV heads in turn
+// (blocks go to the XCDs in turn, so a head's row tiles meet its keys in one
+// L2), then splits, then row tiles from the last, which sees most keys, to the
+// first.  A block takes at most u units.  With items fewer than half the slots
+// u = cost / (slots - items): sum of ceil(units / u) <= cost / u + items <=
+// slots, one round of blocks.  With more, twice a slot's share of the cost, and
+// from the slots' own number on once that share: alike items stay whole, one of
+// a long sequence among short ones does not outlast the others.  Partial
+// results: at most 2 cost / u <= 2 slots, as an item that is split has more
+// than u units.  (The cost is a float sum, taken a little larger.)
+struct Schedule {
+    SeqLen one;          // this lane's sequence, where they are at most 64
+    int per, u;          // sequences a lane, units a block
+    int at, part;        // items and partial results before this lane's sequences
+    int n_item, total;   // items of this lane's sequences, and of all
+};
+__device__ __forceinline__ int splits_of(const Schedule& sc, const SeqLen& l) {
+    return l.units <= sc.u ? 1 : (int)ceilf((float)l.units / (float)sc.u);
+}
+template <bool LONG>
+__device__ __forceinline__ Schedule schedule(const AttnArgs& a, const Part& pt, bool joining) {
     const int lane = threadIdx.x & 63, n_seq = a.r.n_seq, h_kv = a.p.H_kv;
-    const int per = (n_seq + 63) >> 6, s0 = lane * per, s1 = min(s0 + per, n_seq);
-    SeqLen one{};
+    Schedule sc;
+    sc.per = (n_seq + 63) >> 6;
+    const int s0 = lane * sc.per, s1 = min(s0 + sc.per, n_seq);
+    sc.one = SeqLen{};
     int items = 0;
-    long long cost = 0;
+    float cost = 0.0f;
     for (int s = s0; s < s1; s++) {
-        one = seq_len(a, pt, s);
-        items += one.tiles * h_kv;
-        cost += (long long)one.tiles * h_kv * one.units;
+        sc.one = seq_len(a, pt, s);
+        items += sc.one.tiles * h_kv;
+        cost += (float)(sc.one.tiles * h_kv) * (float)sc.one.units;
     }
-    const int all = wave_sum(items);
+    const int all = lane63(scan_add(items));
     const int room = all >= pt.slots ? pt.slots : max(pt.slots - all, pt.slots / 2);
-    const int u = (int)max(1ll, min((wave_sum(cost) + room - 1) / room, 0x7fffffffll));
-    auto splits = [&](const SeqLen& l) { return (int)(((long long)l.units + u - 1) / u); };
-    int parts = 0, found = 0;  // of this lane's sequences
+    const float share = lane63(scan_add(cost)) * 1.00001f / (float)room;
+    sc.u = max(1, (int)fminf(ceilf(share), 1e9f));
+    int n_part = 0, longest = 0;
+    sc.n_item = 0;
     for (int s = s0; s < s1; s++) {
-        if (per > 1) one = seq_len(a, pt, s);
-        const int n = one.tiles * h_kv, sp = splits(one);
-        parts += sp > 1 ? n * sp : 0;
-        found += joining ? (sp > 1 ? n : 0) : n * sp;
+        if (sc.per > 1) sc.one = seq_len(a, pt, s);
+        const int n = sc.one.tiles * h_kv, sp = splits_of(sc, sc.one);
+        n_part += sp > 1 ? n * sp : 0;
+        sc.n_item += joining ? (sp > 1 ? n : 0) : n * sp;
+        if (LONG) longest = (int)((float)sc.one.units / (float)sp);
     }
-    int upto = found, upto_p = parts;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(upto, o, 64), z = __shfl_up(upto_p, o, 64);
-        if (lane >= o) {
-            upto += y;
-            upto_p += z;
+    sc.at = scan_add(sc.n_item);
+    sc.total = lane63(sc.at);
+    sc.at -= sc.n_item;
+    sc.part = scan_add(n_part) - n_part;
+    if (LONG && sc.per == 1 && n_seq > 1) {
+        sc.at = 0;
+        for (int j = 0; j < n_seq; j++) {
+            const int other = __builtin_amdgcn_readlane(longest, j), n = __builtin_amdgcn_readlane(sc.n_item, j);
+            sc.at += other > longest || (other == longest && j < lane) ? n : 0;
         }
     }
-    const unsigned long long past = __ballot(upto > x);
-    if (past == 0) return false;
-    const int owner = __ffsll(past) - 1;
-    // the owner walks its sequences
-    int at = upto - found, part = upto_p - parts, seq = s0;
-    if (lane == owner) {
-        for (int s = s0; s < s1; s++) {
-            if (per > 1) one = seq_len(a, pt, s);
+    return sc;
+}
+// Item x, below sc.total.
+__device__ __forceinline__ Item item_of(const AttnArgs& a, const Part& pt, const Schedule& sc, int x,
+                                        bool joining) {
+    const int lane = threadIdx.x & 63, h_kv = a.p.H_kv;
+    const unsigned long long has = __ballot(sc.at <= x && x < sc.at + sc.n_item);
+    const int owner = __ffsll(has) - 1;
+    SeqLen one = sc.one;
+    int at = sc.at, part = sc.part, seq = lane * sc.per;
+    if (sc.per > 1 && lane == owner) {  // the owner walks its sequences
+        const int s1 = min(seq + sc.per, a.r.n_seq);
+        for (int s = seq; s < s1; s++) {
+            one = seq_len(a, pt, s);
             seq = s;
-            const int n = one.tiles * h_kv, sp = splits(one);
+            const int n = one.tiles * h_kv, sp = splits_of(sc, one);
             const int c = joining ? (sp > 1 ? n : 0) : n * sp;
             if (x < at + c) break;
             at += c;
@@ -207,19 +247,28 @@ __device__ __forceinline__ bool schedule(const AttnArgs& a, const Part& pt, int 
         }
     }
     auto from = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
+    Item it;
     it.seq = from(seq);
     it.row0 = from(one.row0);
     it.n_q = from(one.n_q);
     it.kv = from(one.kv);
-    it.n_split = from(splits(one));
-    const int tiles = from(one.tiles), j = x - from(at);
-    it.head = j % h_kv;
-    const int k = j / h_kv;
-    it.split = joining ? 0 : k % it.n_split;
-    const int q = joining ? k : k / it.n_split;  // row tiles from the last
-    it.qt = tiles - 1 - q;
+    it.n_split = from(splits_of(sc, one));
+    const int tiles = from(one.tiles), j = x - from(at), k = a.by_kv.div(j);
+    it.head = j - k * h_kv;
+    const int q = joining || it.n_split == 1 ? k : (int)((uint32_t)k / (uint32_t)it.n_split);
+    it.split = joining ? 0 : k - q * it.n_split;
+    it.qt = tiles - 1 - q;  // row tiles from the last
     it.part = from(part) + q * it.n_split * h_kv + it.head;
-    return true;
+    return it;
+}
+// Units [lo, hi) of the item's split, of `units`: the first ones have one more.
+__device__ __forceinline__ void split_units(const Item& it, int units, int& lo, int& hi) {
+    lo = 0;
+    hi = units;
+    if (it.n_split == 1) return;
+    const int each = (int)((uint32_t)units / (uint32_t)it.n_split), more = units - each * it.n_split;
+    lo = each * it.split + min(it.split, more);
+    hi = lo + each + (it.split < more ? 1 : 0);
 }
 
 // Tokens that row r of the item's sequence sees.
@@ -265,8 +314,9 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
         float acc[NW][16][LD];
     } lds;
     __shared__ float s_m[NW][16], s_l[NW][16];
-    Item it;
-    if (!schedule(a, pt, blockIdx.x, false, it)) return;
+    const Schedule sc = schedule<false>(a, pt, false);
+    if ((int)blockIdx.x >= sc.total) return;
+    const Item it = item_of(a, pt, sc, blockIdx.x, false);
     const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, li = lane & 15, lg = lane >> 4;
     const int rows = min(16, it.n_q * a.n_rep - it.qt * 16);  // of this tile
     const int r0 = it.qt * 16;
@@ -289,8 +339,10 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
     const int vis = visible(a, it, r0 + min(li, rows - 1));  // (no row: what the last one sees)
     const int vis_lo = visible(a, it, r0), vis_hi = visible(a, it, r0 + rows - 1);
     const int units = (vis_hi + STREAM_UNIT - 1) / STREAM_UNIT;
-    const int t_lo = (int)((long long)units * it.split / it.n_split) * NW;
-    const int t_hi = min((int)((long long)units * (it.split + 1) / it.n_split) * NW, (vis_hi + 31) >> 5);
+    int t_lo, t_hi;
+    split_units(it, units, t_lo, t_hi);
+    t_lo *= NW;
+    t_hi = min(t_hi * NW, (vis_hi + 31) >> 5);
     const float sc2 = score_scale(a.r.scale);
     const T* kp = (const T*)a.p.k;
     const T* vp = (const T*)a.p.v;
@@ -481,11 +533,13 @@ __global__ __launch_bounds__(256) void attn_stream_join_kernel(AttnArgs a, Part 
     typedef float fe __attribute__((ext_vector_type(E)));
     __shared__ float s_o[W > 1 ? W : 1][D];
     __shared__ float2 s_ml[W];
-    Item it;
-    if (!schedule(a, pt, blockIdx.x / (16 / RB), true, it)) return;
+    const Schedule sc = schedule<false>(a, pt, true);
     const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, h_kv = a.p.H_kv;
-    const int row = blockIdx.x % (16 / RB) * RB + wv / W, r = it.qt * 16 + row;
-    if (r >= it.n_q * a.n_rep) return;  // (W > 1: of the whole block)
+    for (int x = blockIdx.x; x < sc.total * (16 / RB); x += gridDim.x) {
+    const Item it = item_of(a, pt, sc, x / (16 / RB), true);
+    const int row = x % (16 / RB) * RB + wv / W, r = it.qt * 16 + row;
+    if (r >= it.n_q * a.n_rep) continue;  // (W > 1: of the whole block)
+    if (W > 1) __syncthreads();           // the last row's sums are read
     float* ws = static_cast<float*>(a.r.ws);
     const int tok = a.by_rep.div(r), hq = it.head * a.n_rep + r - tok * a.n_rep;
     fe o = {};
@@ -493,12 +547,12 @@ __global__ __launch_bounds__(256) void attn_stream_join_kernel(AttnArgs a, Part 
     // eight splits in flight, their maxima with them
     for (int i0 = wv % W; i0 < it.n_split; i0 += 8 * W) {
         float2 ml[8];
-        fe x[8];
+        fe v[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int i = min(i0 + j * W, it.n_split - 1);
             ml[j] = part_ml(ws, pt, D, it.part + i * h_kv)[row];
-            x[j] = *reinterpret_cast<const fe*>(part_acc(ws, pt, D, it.part + i * h_kv) + row * D + E * lane);
+            v[j] = *reinterpret_cast<const fe*>(part_acc(ws, pt, D, it.part + i * h_kv) + row * D + E * lane);
         }
         float top = m;
 #pragma unroll
@@ -512,7 +566,7 @@ __global__ __launch_bounds__(256) void attn_stream_join_kernel(AttnArgs a, Part 
             if (i0 + j * W >= it.n_split) break;
             const float f = __builtin_amdgcn_exp2f(ml[j].x - m);
             l += ml[j].y * f;
-            o += x[j] * f;
+            o += v[j] * f;
         }
     }
     if constexpr (W > 1) {
@@ -520,7 +574,7 @@ __global__ __launch_bounds__(256) void attn_stream_join_kernel(AttnArgs a, Part 
         for (int e = 0; e < E; e++) s_o[wv][E * lane + e] = o[e];
         if (lane == 0) s_ml[wv] = float2{m, l};
         __syncthreads();
-        if (wv > 0) return;
+        if (wv > 0) continue;
         m = fmaxf(fmaxf(s_ml[0].x, s_ml[1].x), fmaxf(s_ml[2].x, s_ml[3].x));
         l = 0.0f;
         o = fe{};
@@ -537,6 +591,7 @@ __global__ __launch_bounds__(256) void attn_stream_join_kernel(AttnArgs a, Part 
     T* out = (T*)a.r.out + (it.row0 + tok) * a.r.out_token + hq * a.r.out_head + E * lane;
 #pragma unroll
     for (int e = 0; e < E; e++) out[e] = (T)(o[e] * inv * (a.r.gate ? sigmoid(gate[e]) : 1.0f));
+    }
 }
 
 // ------------------------------------------------------------ many rows
@@ -614,7 +669,7 @@ template <typename T, int D, int KG>
 __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) {
     constexpr int NS = D / 16, ND = D / 32;  // K steps of a score, dim tiles
     constexpr int ROW = 2 * D, SLOT = 64 * ROW;  // bytes
-    constexpr int CH = D / 8, KPI = 64 / CH, NL = 16 / KPI;  // pieces a row, keys a load, loads of 16 keys
+    constexpr int CH = D / 8, KPI = 64 / CH, NL = 8 / KPI;  // pieces a row, keys a load, loads of 8 keys
     constexpr int AHEAD = D == 64 ? 4 : D == 128 ? 6 : 3;
     // Q operands that stay in LDS: a register file holds 128 of O, 64 of Q, 16
     // scores and 16 of operands, and a few too few for what goes with them.
@@ -626,8 +681,9 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
     long long* const tab = reinterpret_cast<long long*>(lds + 4 * SLOT);
     __shared__ int s_bad;
     __shared__ float2 s_ml[2][4][32];
-    Item it;
-    if (!schedule(a, pt, blockIdx.x, false, it)) return;
+    const Schedule sc = schedule<true>(a, pt, false);
+    if ((int)blockIdx.x >= sc.total) return;
+    const Item it = item_of(a, pt, sc, blockIdx.x, false);
     const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int ln = lane & 31, hh = lane >> 5;
     const int rg = KG == 1 ? wv : wv & 3, kg = KG == 1 ? 0 : wv >> 2;
@@ -638,8 +694,8 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
     const int vis = visible(a, it, r_in);
     const int vis_hi = visible(a, it, min(it.qt * BR + BR, n_rows) - 1);
     const int units = (vis_hi + 63) >> 6;
-    const int u_lo = (int)((long long)units * it.split / it.n_split);
-    const int u_hi = (int)((long long)units * (it.split + 1) / it.n_split);
+    int u_lo, u_hi;
+    split_units(it, units, u_lo, u_hi);
     x8 qb[NS - QL];
     char* const ql = lds + 4 * SLOT + TAB * (int)sizeof(long long) + wv * (QL * 1024) + lane * 16;
     {
@@ -668,37 +724,39 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
             if (bad) s_bad = 1;
         }
     };
-    // A unit into a slot, by wavefronts 4 to 7: 16 keys each, NL loads of 1 KB of
-    // K and of V.  A load takes the address unit 16 cycles, and a wavefront
-    // waits where others' are before its own: while these four do, the other
-    // wavefront of each SIMD has the matrix cores, and they have them while it
-    // takes its weights.  Where the 16 keys lie in one page, as they do in pages
-    // of a multiple of 16, an address is a scalar and a lane's constant; else
-    // each lane looks its key up.
+    // A unit into a slot: 8 keys a wavefront, NL loads of 1 KB of K and of V.  A
+    // load takes the address unit 16 cycles, and a wavefront waits where others'
+    // are before its own.  So the two wavefronts of a SIMD, i and i + 4, take
+    // turns: i + 4 loads while i has the matrix cores for its scores, and i
+    // loads while i + 4 has them (all eight at once, or between their products,
+    // left the matrix cores idle half the time: 890 us of 8,192 tokens, not 8).
+    // Where the 8 keys lie in one page, as they do in pages of a multiple of 8,
+    // an address is a scalar and a lane's constant; else each lane looks its
+    // key up.
     const char* const kh = (const char*)a.p.k + 2 * (it.head * a.p.head_stride);
     const char* const vh = (const char*)a.p.v + 2 * (it.head * a.p.head_stride);
     const int last = vis_hi - 1;
-    const bool by_group = a.p.page_size % 16 == 0 && a.p.token_stride * a.p.page_size < 1 << 28;
+    const bool by_group = a.p.page_size % 8 == 0 && a.p.token_stride * a.p.page_size < 1 << 28;
     auto stage = [&](int u) __attribute__((always_inline)) {
-        const int w = wv & 3, l = lane_again(), lk = l / CH, p = l % CH;
-        const uint32_t to = ((u - u_lo) & 1) * SLOT + w * NL * 1024;
+        const int l = lane_again(), lk = l / CH, p = l % CH;
+        const uint32_t to = ((u - u_lo) & 1) * SLOT + wv * NL * 1024;
         auto piece_k = [&](int key) { return (p ^ (D == 64 ? (key >> 1) & 7 : key & 15)) << 4; };
         auto piece_v = [&](int key) { return (p ^ (D == 64 ? (key & 2) << 1 : (key & 3) << 2)) << 4; };
         if (by_group) {
-            const int t = min(u * 64 + w * 16, last & ~15), pg = a.by_page.div(t);
+            const int t = min(u * 64 + wv * 8, last & ~7), pg = a.by_page.div(t);
             const int ts2 = 2 * (int)a.p.token_stride;
             const long long at = uniform(max(uniform(tab[pg - w0]), 0ll) + (t - pg * a.p.page_size) * ts2);
             const int most = last - t;
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                const int row = i * KPI + lk, key = w * 16 + row, off = min(row, most) * ts2;
+                const int row = i * KPI + lk, key = wv * 8 + row, off = min(row, most) * ts2;
                 load_lds16(kh + at, off + piece_k(key), lds_addr(ks) + to + i * 1024);
                 load_lds16(vh + at, off + piece_v(key), lds_addr(vs) + to + i * 1024);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                const int key = w * 16 + i * KPI + lk, t = min(u * 64 + key, last), pg = a.by_page.div(t);
+                const int key = wv * 8 + i * KPI + lk, t = min(u * 64 + key, last), pg = a.by_page.div(t);
                 const long long off = max(tab[pg - w0], 0ll) + 2 * ((t - pg * a.p.page_size) * a.p.token_stride);
                 load_lds16(kh + off + piece_k(key), lds_addr(ks) + to + i * 1024);
                 load_lds16(vh + off + piece_v(key), lds_addr(vs) + to + i * 1024);
@@ -721,7 +779,7 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
     if (u_lo < u_hi) {
         fill(u_lo);
         __syncthreads();
-        if (wv >= 4) stage(u_lo);
+        stage(u_lo);
     }
     // unit u is waited for, the next one started
     auto begin = [&](int u) __attribute__((always_inline)) {
@@ -737,6 +795,7 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
     };
     auto keys = [&](int u, auto masked) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
+        bool staged = wv >= 4 || u + 1 >= u_hi;
 #pragma unroll 1
         for (int sub = kg; sub < 2; sub += KG) {
             const int key0 = u * 64 + 32 * sub;
@@ -769,6 +828,10 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
                 sc = mfma32(kf[st % (AHEAD + 1)],
                             st < QL ? *reinterpret_cast<const x8*>(lds + q_at + st * 1024) : qb[max(st - QL, 0)], sc);
                 __builtin_amdgcn_sched_barrier(0);
+            }
+            if (!staged) {
+                stage(u + 1);
+                staged = true;
             }
             bool odd = false;  // values that are no numbers where a row's mask has to hold
             if constexpr (MASKED) {
@@ -845,7 +908,9 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        if (MASKED && !staged) stage(u + 1);
     };
+    if (wv >= 4) __builtin_amdgcn_s_setprio(1);
     // units that every row sees whole, then the others; all from the first entry
     // outside the cache on
     const int u_mid = min(u_hi, visible(a, it, it.qt * BR) >> 6);
@@ -974,23 +1039,24 @@ template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_tile_join_kernel(AttnArgs a, Part pt) {
     constexpr int ND = D / 32;
     const int groups = pt.rows / 32;
-    Item it;
-    if (!schedule(a, pt, blockIdx.x / (groups * ND), true, it)) return;
-    const int rg = blockIdx.x / ND % groups, i = blockIdx.x % ND;
+    const Schedule sc = schedule<false>(a, pt, true);
     const int q = threadIdx.x >> 6, lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5;
+    for (int x = blockIdx.x; x < sc.total * groups * ND; x += gridDim.x) {
+    const Item it = item_of(a, pt, sc, x / (groups * ND), true);
+    const int rg = x / ND % groups, i = x % ND;
     const int r = it.qt * pt.rows + rg * 32 + ln, h_kv = a.p.H_kv;
-    if (r >= it.n_q * a.n_rep) return;
+    if (r >= it.n_q * a.n_rep) continue;
     float* ws = static_cast<float*>(a.r.ws);
     f4 o = {};
     float m = M_NONE, l = 0.0f;
     for (int s0 = 0; s0 < it.n_split; s0 += 8) {
         float2 ml[8];
-        f4 x[8];
+        f4 v[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int s = min(s0 + j, it.n_split - 1);
             ml[j] = part_ml(ws, pt, D, it.part + s * h_kv)[rg * 32 + ln];
-            x[j] = reinterpret_cast<const f4*>(part_acc(ws, pt, D, it.part + s * h_kv))[((rg * ND + i) * 4 + q) * 64 + lane];
+            v[j] = reinterpret_cast<const f4*>(part_acc(ws, pt, D, it.part + s * h_kv))[((rg * ND + i) * 4 + q) * 64 + lane];
         }
         float top = m;
 #pragma unroll
@@ -1004,11 +1070,12 @@ __global__ __launch_bounds__(256) void attn_tile_join_kernel(AttnArgs a, Part pt
             if (s0 + j >= it.n_split) break;
             const float f = __builtin_amdgcn_exp2f(ml[j].x - m);
             l += ml[j].y * f;
-            o += x[j] * f;
+            o += v[j] * f;
         }
     }
     const float inv = visible(a, it, r) > 0 ? 1.0f / l : 0.0f;
     store_row4<T>(a, it, r, 32 * i + 8 * q + 4 * hh, o * inv);
+    }
 }
 
 // What a call of these sizes launches.
@@ -1051,7 +1118,7 @@ hipError_t launch_tile(const AttnArgs& a, const Plan& p, hipStream_t st) {
     const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(attn_tile_kernel<T, D, KG>), bytes);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((attn_tile_kernel<T, D, KG>), dim3(p.tile_blocks), dim3(512), bytes, st, a, p.pl);
-    hipLaunchKernelGGL((attn_tile_join_kernel<T, D>), dim3(p.tile_joins * (p.pl.rows / 32) * (D / 32)),
+    hipLaunchKernelGGL((attn_tile_join_kernel<T, D>), dim3(std::min(2048, p.tile_joins * (p.pl.rows / 32) * (D / 32))),
                        dim3(256), 0, st, a, p.pl);
     return hipGetLastError();
 }
@@ -1072,7 +1139,7 @@ hipError_t launch(const AttnArgs& a, hipStream_t st) {
             hipLaunchKernelGGL((attn_stream_join_kernel<T, D, 4>), dim3(p.stream_joins * 16), dim3(256), 0, st,
                                a, p.ps);
         else
-            hipLaunchKernelGGL((attn_stream_join_kernel<T, D, 1>), dim3(p.stream_joins * 4), dim3(256), 0, st, a,
+            hipLaunchKernelGGL((attn_stream_join_kernel<T, D, 1>), dim3(std::min(2048, p.stream_joins * 4)), dim3(256), 0, st, a,
                                p.ps);
     }
     return hipGetLastError();

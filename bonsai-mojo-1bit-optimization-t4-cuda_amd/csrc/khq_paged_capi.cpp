@@ -106,6 +106,7 @@ int khq_paged_attn(const khq_attn_rows* rows, const khq_pages* pages, hipStream_
     a.n_rep = r.H_q / pages->H_kv;
     a.by_page = khq::FastDiv(pages->page_size);
     a.by_rep = khq::FastDiv(a.n_rep);
+    a.by_kv = khq::FastDiv(pages->H_kv);
     const size_t need = khq::paged::attn_ws_bytes(r.n_tok, r.n_seq, r.H_q, pages->H_kv,
                                                   pages->head_dim, r.max_q);
     if (r.ws) {

@@ -43,7 +43,7 @@ struct AttnArgs {
     khq_attn_rows r;  // ws set
     khq_pages p;
     int n_rep;
-    FastDiv by_page, by_rep;  // page_size, n_rep
+    FastDiv by_page, by_rep, by_kv;  // page_size, n_rep, H_kv
 };
 hipError_t launch_attn(const AttnArgs& a, hipStream_t st);
 size_t attn_ws_bytes(int n_tok, int n_seq, int H_q, int H_kv, int head_dim, int max_q);
