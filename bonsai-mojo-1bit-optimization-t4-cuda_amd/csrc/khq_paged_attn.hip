@@ -66,18 +66,18 @@ __device__ __forceinline__ float add_pair(uint32_t p, float l) {
         return l + ((float)v[0] + (float)v[1]);
     }
 }
-// Whether either 16-bit value of a pair is an infinity or a NaN.
+// A pair with infinities and NaN as the type's largest values: a weight of 0
+// makes a 0 of them.
 template <typename T>
-__device__ __forceinline__ bool nonfinite_pair(uint32_t p) {
-    const uint32_t e = __is_same(T, fp16) ? 0x7c00u : 0x7f80u;
-    return (p & e) == e || (p & (e << 16)) == (e << 16);
+__device__ __forceinline__ uint32_t finite_pair(uint32_t p) {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    const unsigned short top = __is_same(T, fp16) ? 0x7bff : 0x7f7f;
+    const us2 size = __builtin_elementwise_min(__builtin_bit_cast(us2, p & 0x7fff7fffu), us2{top, top});
+    return (p & 0x80008000u) | __builtin_bit_cast(uint32_t, size);
 }
 template <typename T>
-__device__ __forceinline__ uint32_t finite_pair(uint32_t p) {  // those as zeros
-    const uint32_t e = __is_same(T, fp16) ? 0x7c00u : 0x7f80u;
-    if ((p & e) == e) p &= 0xffff0000u;
-    if ((p & (e << 16)) == (e << 16)) p &= 0xffffu;
-    return p;
+__device__ __forceinline__ bool nonfinite_pair(uint32_t p) {
+    return finite_pair<T>(p) != p;
 }
 template <typename T>
 __device__ __forceinline__ float sigmoid(T g) {
@@ -696,22 +696,6 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
     const int units = (vis_hi + 63) >> 6;
     int u_lo, u_hi;
     split_units(it, units, u_lo, u_hi);
-    x8 qb[NS - QL];
-    char* const ql = lds + 4 * SLOT + TAB * (int)sizeof(long long) + wv * (QL * 1024) + lane * 16;
-    {
-        const uint32_t flip = a.r.scale < 0.0f ? 0x80008000u : 0u;
-        const int tok = a.by_rep.div(r_in);
-        const T* q = (const T*)a.r.q + (it.row0 + tok) * a.r.q_token +
-                     (it.head * a.n_rep + r_in - tok * a.n_rep) * a.r.q_head + 8 * hh;
-#pragma unroll
-        for (int st = 0; st < NS; st++) {
-            const u4e v = *reinterpret_cast<const u4e*>(q + 16 * st);
-            const u4 w = {v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip};
-            if (st < QL) *reinterpret_cast<u4*>(ql + st * 1024) = w;
-            else qb[st - QL] = __builtin_bit_cast(x8, w);
-        }
-    }
-    const int q_at = lds_addr(ql) - lds_addr(lds);
     const float sc2 = score_scale(a.r.scale);
     int w0 = 0;  // first page of the table's window
     auto fill = [&](int u) __attribute__((always_inline)) {
@@ -781,6 +765,22 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
         __syncthreads();
         stage(u_lo);
     }
+    x8 qb[NS - QL];
+    char* const ql = lds + 4 * SLOT + TAB * (int)sizeof(long long) + wv * (QL * 1024) + lane * 16;
+    {
+        const uint32_t flip = a.r.scale < 0.0f ? 0x80008000u : 0u;
+        const int tok = a.by_rep.div(r_in);
+        const T* q = (const T*)a.r.q + (it.row0 + tok) * a.r.q_token +
+                     (it.head * a.n_rep + r_in - tok * a.n_rep) * a.r.q_head + 8 * hh;
+#pragma unroll
+        for (int st = 0; st < NS; st++) {
+            const u4e v = *reinterpret_cast<const u4e*>(q + 16 * st);
+            const u4 w = {v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip};
+            if (st < QL) *reinterpret_cast<u4*>(ql + st * 1024) = w;
+            else qb[st - QL] = __builtin_bit_cast(x8, w);
+        }
+    }
+    const int q_at = lds_addr(ql) - lds_addr(lds);
     // unit u is waited for, the next one started
     auto begin = [&](int u) __attribute__((always_inline)) {
         wait_loads();
@@ -845,6 +845,7 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
 #pragma unroll
                 for (int e = 0; e < 16; e++)
                     if (key0 + 8 * (e >> 2) + 4 * hh + (e & 3) >= vis) sc[e] = -INFINITY;
+#pragma unroll 4
                 for (int i = 0; i < D / 16; i++) {
                     const u4 v = *reinterpret_cast<const u4*>(vb + (i * 64 + lane) * 16);
                     odd = odd || nonfinite_pair<T>(v.x) || nonfinite_pair<T>(v.y) ||
@@ -902,7 +903,7 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
                 if (n + AHEAD < 2 * ND) read_v(n + AHEAD);
                 __builtin_amdgcn_sched_barrier(0);
                 u4 v = vf[n % (AHEAD + 1)];
-                if (MASKED && odd)  // ... and leave the product
+                if constexpr (MASKED)  // ... and leave the product
                     v = u4{finite_pair<T>(v.x), finite_pair<T>(v.y), finite_pair<T>(v.z), finite_pair<T>(v.w)};
                 acc[n >> 1] = mfma32(__builtin_bit_cast(x8, v), pb[n & 1], acc[n >> 1]);
                 __builtin_amdgcn_sched_barrier(0);
@@ -927,26 +928,38 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
         keys(u, std::true_type{});
     }
     float l_row = l_part + __shfl_xor(l_part, 32, 64);
-    __syncthreads();  // the slots are free: 32 rows of half the dims for each wavefront
     constexpr int HD = ND / 2, AREA = 32 * (D / 2) * (int)sizeof(float);
     const int el = lane_again(), eln = el & 31, ehh = el >> 5;
-    // ---- dims dim0 + 32 i + 8 q + 4 ehh + c of row eln leave
+    __syncthreads();  // the slots are free: 32 rows of half the dims for each wavefront
+    // Half `half` of the dims: dim 32 i + 8 q + 4 ehh + c of it of row eln in
+    // res[i][4 q + c].  (Code that runs once a block costs more to fetch than to
+    // run: the halves are a loop, and a row's place is computed by one lane.)
+    auto leave_part = [&](const f16v(&res)[HD], int half) __attribute__((always_inline)) {
+        float* ws = static_cast<float*>(a.r.ws);
+        const int part = it.part + it.split * a.p.H_kv;
+        f4* const x = reinterpret_cast<f4*>(part_acc(ws, pt, D, part)) + (rg * ND + half * HD) * (4 * 64) + el;
+#pragma unroll
+        for (int i = 0; i < HD; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                x[(i * 4 + q) * 64] = f4{res[i][4 * q], res[i][4 * q + 1], res[i][4 * q + 2], res[i][4 * q + 3]};
+        if (ehh == 0 && half == 0) part_ml(ws, pt, D, part)[rg * 32 + eln] = float2{m_ref, l_row};
+    };
+    // Outputs go through LDS, so that a lane stores 16 bytes next to its
+    // neighbours': lane el takes 8-dim group el % GN of row el / GN of RI at once.
     auto leave = [&](const f16v(&res)[HD], int half, char* area) __attribute__((always_inline)) {
-        const int r0 = it.qt * BR + rg * 32;
-        if (it.n_split > 1) {
-            float* ws = static_cast<float*>(a.r.ws);
-            const int part = it.part + it.split * a.p.H_kv;
-            f4* const x = reinterpret_cast<f4*>(part_acc(ws, pt, D, part)) + (rg * ND + half * HD) * (4 * 64) + el;
+        constexpr int CN = D / 8, GN = D / 16, RI = 64 / GN, NR = 32 / RI;
+        const int r0 = it.qt * BR + rg * 32, r = min(r0 + eln, n_rows - 1), tok = a.by_rep.div(r);
+        const int hq = it.head * a.n_rep + r - tok * a.n_rep;
+        const long long to = (it.row0 + tok) * a.r.out_token + hq * a.r.out_head;
+        const long long gt = (it.row0 + tok) * a.r.gate_token + hq * a.r.gate_head;
+        const int g = el % GN, dim = half * (D / 2) + 8 * g;
+        u4 gate[NR];
+        if (a.r.gate) {
 #pragma unroll
-            for (int i = 0; i < HD; i++)
-#pragma unroll
-                for (int q = 0; q < 4; q++)
-                    x[(i * 4 + q) * 64] = f4{res[i][4 * q], res[i][4 * q + 1], res[i][4 * q + 2], res[i][4 * q + 3]};
-            if (ehh == 0 && half == 0) part_ml(ws, pt, D, part)[rg * 32 + eln] = float2{m_ref, l_row};
-            return;
+            for (int k = 0; k < NR; k++)
+                gate[k] = *reinterpret_cast<const u4e*>((const T*)a.r.gate + __shfl(gt, k * RI + el / GN, 64) + dim);
         }
-        // through LDS, so that a lane stores 16 bytes next to its neighbours'
-        constexpr int CN = D / 8, GN = D / 16, RI = 64 / GN;  // pieces and 8-dim groups of a half row, rows at once
         const float inv = vis > 0 ? 1.0f / l_row : 0.0f;
         mu::wave_sync();
 #pragma unroll
@@ -956,47 +969,39 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
                 *reinterpret_cast<f4*>(area + eln * (CN * 16) + (((8 * i + 2 * q + ehh) ^ (eln & (CN - 1))) << 4)) =
                     f4{res[i][4 * q], res[i][4 * q + 1], res[i][4 * q + 2], res[i][4 * q + 3]} * inv;
         mu::wave_sync();
-        const int g = el % GN, dim = half * (D / 2) + 8 * g;
-        u4 gate[32 / RI];
-        T* out[32 / RI];
 #pragma unroll
-        for (int k = 0; k < 32 / RI; k++) {
-            const int r = r0 + k * RI + el / GN, rr = min(r, n_rows - 1), tok = a.by_rep.div(rr);
-            const int hq = it.head * a.n_rep + rr - tok * a.n_rep;
-            out[k] = r < n_rows ? (T*)a.r.out + (it.row0 + tok) * a.r.out_token + hq * a.r.out_head + dim : nullptr;
-            gate[k] = u4{0u, 0u, 0u, 0u};
-            if (a.r.gate)
-                gate[k] = *reinterpret_cast<const u4e*>((const T*)a.r.gate + (it.row0 + tok) * a.r.gate_token +
-                                                        hq * a.r.gate_head + dim);
-        }
-#pragma unroll
-        for (int k = 0; k < 32 / RI; k++) {
+        for (int k = 0; k < NR; k++) {
             const int row = k * RI + el / GN, s = row & (CN - 1);
-            const f4 x = *reinterpret_cast<const f4*>(area + row * (CN * 16) + (((2 * g) ^ s) << 4));
-            const f4 y = *reinterpret_cast<const f4*>(area + row * (CN * 16) + (((2 * g + 1) ^ s) << 4));
-            float o[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            f4 x = *reinterpret_cast<const f4*>(area + row * (CN * 16) + (((2 * g) ^ s) << 4));
+            f4 y = *reinterpret_cast<const f4*>(area + row * (CN * 16) + (((2 * g + 1) ^ s) << 4));
             if (a.r.gate) {
                 const x8 gv = __builtin_bit_cast(x8, gate[k]);
 #pragma unroll
-                for (int e = 0; e < 8; e++) o[e] *= sigmoid(gv[e]);
+                for (int e = 0; e < 4; e++) {
+                    x[e] *= sigmoid(gv[e]);
+                    y[e] *= sigmoid(gv[4 + e]);
+                }
             }
-            if (out[k])
-                *reinterpret_cast<u4e*>(out[k]) = u4e{pack<T>(o[0], o[1]), pack<T>(o[2], o[3]),
-                                                      pack<T>(o[4], o[5]), pack<T>(o[6], o[7])};
+            const long long o = __shfl(to, row, 64);
+            if (r0 + row < n_rows)
+                *reinterpret_cast<u4e*>((T*)a.r.out + o + dim) =
+                    u4e{pack<T>(x[0], x[1]), pack<T>(x[2], x[3]), pack<T>(y[0], y[1]), pack<T>(y[2], y[3])};
         }
     };
+    f16v res[HD];
     if constexpr (KG == 1) {
-        f16v res[HD];
 #pragma unroll
+        for (int i = 0; i < HD; i++) res[i] = acc[i];
+#pragma unroll 1
         for (int half = 0; half < 2; half++) {
+            if (it.n_split == 1) leave(res, half, lds + wv * AREA);
+            else leave_part(res, half);
 #pragma unroll
-            for (int i = 0; i < HD; i++) res[i] = acc[half * HD + i];
-            leave(res, half, lds + wv * AREA);
+            for (int i = 0; i < HD; i++) res[i] = acc[HD + i];
         }
     } else {
         // the two halves of a row's keys: wavefront kg joins and stores half kg of the dims
-        f16v res[HD];
-        auto give = [&](const f16v* from) {
+        auto give = [&](const f16v* from) __attribute__((always_inline)) {
             f4* const x = reinterpret_cast<f4*>(lds + (rg * 2 + kg) * AREA) + el;
 #pragma unroll
             for (int i = 0; i < HD; i++)
@@ -1030,7 +1035,8 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
 #pragma unroll
                 for (int c = 0; c < 4; c++) res[i][4 * q + c] = res[i][4 * q + c] * f1 + o[c] * f2;
             }
-        leave(res, kg, area);
+        if (it.n_split == 1) leave(res, kg, area);
+        else leave_part(res, kg);
     }
 }
 
