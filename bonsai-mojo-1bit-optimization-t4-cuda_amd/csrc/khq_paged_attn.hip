@@ -11,8 +11,8 @@
 //
 // Two kernels share the sequences by their row count: up to 16 rows (a decode
 // step's 6 of 24 / 4 heads) stream keys and values through registers
-// (attn_stream_kernel), more go in tiles of 128 or 256 rows that share keys
-// and values in LDS (attn_tile_kernel).
+// (stream_item), more go in tiles of 128 or 256 rows that share keys
+// and values in LDS (tile_item).
 #include "khq_mfma_util.h"
 #include "khq_paged_internal.h"
 
@@ -101,11 +101,10 @@ __device__ __forceinline__ float score_scale(float scale) {
 
 // ------------------------------------------------------------ the partition
 constexpr int SMALL_ROWS = 16;
-constexpr int STREAM_WAVES = 4;
-constexpr int STREAM_UNIT = 32 * STREAM_WAVES;  // keys: a 32-key tile for each wavefront
-constexpr int STREAM_SLOTS = 512;               // blocks that run at once, two a CU
+// Blocks of the stream kernel: 4 wavefronts, two blocks a CU; 8 and one where
+// they share a launch with tiles.  A unit is a 32-key tile for each wavefront.
+constexpr int STREAM_WAVES = 4, STREAM_SLOTS = 512;
 constexpr int TILE_UNIT = 64;
-constexpr int TILE_SLOTS = 256;
 
 // Which sequences a launch serves: by their rows, or all of them.
 enum Serve { SERVE_SMALL, SERVE_LARGE, SERVE_ALL };
@@ -115,6 +114,7 @@ struct Part {
     int unit;   // keys
     int slots;  // blocks
     Serve serve;
+    size_t at;  // of its partial results in the workspace, in floats
 };
 
 struct Item {
@@ -129,9 +129,9 @@ struct SeqLen {
 
 __device__ __forceinline__ SeqLen seq_len(const AttnArgs& a, const Part& pt, int s) {
     SeqLen l;
-    const int c0 = min(max(a.r.cu_q[s], 0), a.r.n_tok), c1 = min(max(a.r.cu_q[s + 1], 0), a.r.n_tok);
+    const int c0 = a.r.cu_q[s], c1 = min(a.r.cu_q[s + 1], a.r.n_tok);
     l.row0 = c0;
-    l.n_q = max(c1 - c0, 0);
+    l.n_q = c0 >= 0 ? max(c1 - min(c0, a.r.n_tok), 0) : 0;  // none from outside the batch
     l.kv = min(max(a.r.seq_kv[s], 0), a.r.table_ld * a.p.page_size);
     const int rows = l.n_q * a.n_rep;
     const bool mine = pt.serve == SERVE_ALL || (rows <= SMALL_ROWS) == (pt.serve == SERVE_SMALL);
@@ -287,11 +287,23 @@ __device__ __forceinline__ long long token_at(const AttnArgs& a, const Item& it,
 
 // Partial results: f32 [2 slots][rows][D] (each kernel's own order of one's
 // values), then (maximum, sum) f32 pairs [2 slots][rows].
-__device__ __forceinline__ float* part_acc(float* ws, const Part& pt, int d, int part) {
-    return ws + (size_t)part * pt.rows * d;
+__device__ __forceinline__ float* part_acc(const AttnArgs& a, const Part& pt, int d, int part) {
+    return static_cast<float*>(a.r.ws) + pt.at + (size_t)part * pt.rows * d;
 }
-__device__ __forceinline__ float2* part_ml(float* ws, const Part& pt, int d, int part) {
-    return reinterpret_cast<float2*>(ws + (size_t)2 * pt.slots * pt.rows * d) + (size_t)part * pt.rows;
+__device__ __forceinline__ float2* part_ml(const AttnArgs& a, const Part& pt, int d, int part) {
+    return reinterpret_cast<float2*>(static_cast<float*>(a.r.ws) + pt.at + (size_t)2 * pt.slots * pt.rows * d) +
+           (size_t)part * pt.rows;
+}
+
+// x, of which the compiler knows nothing: what follows from it is computed where
+// it is used, and not kept in registers that there are not.
+__device__ __forceinline__ int opaque(int x) {
+    asm("" : "+v"(x));
+    return x;
+}
+__device__ __forceinline__ long long uniform(long long x) {
+    const int lo = __builtin_amdgcn_readfirstlane((int)x), hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
+    return ((long long)hi << 32) | (uint32_t)lo;
 }
 
 // ------------------------------------------------------------ few rows
@@ -303,20 +315,17 @@ __device__ __forceinline__ float2* part_ml(float* ws, const Part& pt, int d, int
 // a lane loads those 8 keys' values of 8 consecutive dims and transposes them
 // in its registers (32 byte permutes), dim 8 m + t standing for row m of
 // product t.  No LDS and no barrier until the block's wavefronts join.
-template <typename T, int D>
-__global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnArgs a, Part pt) {
-    constexpr int NW = STREAM_WAVES, KS = D / 32;          // K steps of a score
+template <typename T, int D, int NW>
+__device__ __forceinline__ void stream_item(const AttnArgs& a, const Part& pt, const Item& it, char* smem) {
+    constexpr int KS = D / 32;                             // K steps of a score
     constexpr int VE = D == 64 ? 4 : 8, NH = D / 16 / VE;  // dims a lane loads at once, times
     constexpr int LD = D + 4;
     typedef typename V<T>::x8 x8;
-    __shared__ union __align__(16) {
+    struct Lds {
+        float acc[NW][16][LD], m[NW][16], l[NW][16];
         T q[16][D + 8];
-        float acc[NW][16][LD];
-    } lds;
-    __shared__ float s_m[NW][16], s_l[NW][16];
-    const Schedule sc = schedule<false>(a, pt, false);
-    if ((int)blockIdx.x >= sc.total) return;
-    const Item it = item_of(a, pt, sc, blockIdx.x, false);
+    };
+    Lds& lds = *reinterpret_cast<Lds*>(smem);
     const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, li = lane & 15, lg = lane >> 4;
     const int rows = min(16, it.n_q * a.n_rep - it.qt * 16);  // of this tile
     const int r0 = it.qt * 16;
@@ -333,12 +342,18 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
         *reinterpret_cast<u4*>(&lds.q[row][8 * c]) = u4{v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip};
     }
     __syncthreads();
+    // (256 dims: 32 registers of them, and as many too few for all of a tile's
+    // loads at once; they are read again for each tile)
     x8 qf[KS];
+    auto read_q = [&]() {
+        const T* q = &lds.q[0][0] + opaque(li * (D + 8) + 8 * lg);
 #pragma unroll
-    for (int st = 0; st < KS; st++) qf[st] = *reinterpret_cast<const x8*>(&lds.q[li][32 * st + 8 * lg]);
+        for (int st = 0; st < KS; st++) qf[st] = *reinterpret_cast<const x8*>(q + 32 * st);
+    };
+    if (D < 256) read_q();
     const int vis = visible(a, it, r0 + min(li, rows - 1));  // (no row: what the last one sees)
     const int vis_lo = visible(a, it, r0), vis_hi = visible(a, it, r0 + rows - 1);
-    const int units = (vis_hi + STREAM_UNIT - 1) / STREAM_UNIT;
+    const int units = (vis_hi + 32 * NW - 1) / (32 * NW);
     int t_lo, t_hi;
     split_units(it, units, t_lo, t_hi);
     t_lo *= NW;
@@ -352,34 +367,58 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
 #pragma unroll
         for (int t = 0; t < VE; t++) acc[h][t] = f4{0.f, 0.f, 0.f, 0.f};
     float m_ref = M_NONE, l_part = 0.0f;
+    // The block table's entries are read a tile ahead.  In pages of a multiple of
+    // 32 tokens a tile lies in one: addresses are a scalar and 32 bits of a lane's.
+    const bool by_tile = a.p.page_size % 32 == 0 && a.p.token_stride * a.p.page_size < 1 << 28;
+    const int last = vis_hi - 1, ts = (int)a.p.token_stride;
+    auto entry_of = [&](int t) {
+        return a.r.table[(size_t)it.seq * a.r.table_ld + a.by_page.div(min(t * 32 + (lane & 31), last))];
+    };
+    int entry = t_lo + wv < t_hi ? entry_of(t_lo + wv) : 0;
     for (int t = t_lo + wv; t < t_hi; t += NW) {
         const int key0 = t * 32;
         // a lane's key: tokens past the last one seen stand for it
-        bool bad;
-        const long long off = token_at(a, it, min(key0 + (lane & 31), vis_hi - 1), bad);
+        const int tok = min(key0 + (lane & 31), last), in = tok - a.by_page.div(tok) * a.p.page_size;
+        const bool bad = (unsigned)entry >= (unsigned)a.p.n_pages;
         const unsigned long long bad_keys = __ballot(bad);
+        const int page = bad ? 0 : entry;
+        const long long off = page * a.p.page_stride + in * a.p.token_stride + it.head * a.p.head_stride;
+        if (t + NW < t_hi) entry = entry_of(t + NW);
         u4 kr[2][KS];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const T* src = kp + __shfl(off, 16 * h + li, 64) + 8 * lg;
-#pragma unroll
-            for (int st = 0; st < KS; st++) kr[h][st] = *reinterpret_cast<const u4*>(src + 32 * st);
-        }
         uint32_t vr[8][NH][VE / 2];
+        auto loads = [&](auto k_row, auto v_row) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const T* src = vp + __shfl(off, (j & 4) * 4 + 4 * lg + (j & 3), 64) + VE * li;
+            for (int h = 0; h < 2; h++) {
+                const T* src = k_row(16 * h + li);
 #pragma unroll
-            for (int h = 0; h < NH; h++) {
-                if constexpr (VE == 8) {
-                    const u4 v = *reinterpret_cast<const u4*>(src + 128 * h);
-                    vr[j][h][0] = v.x; vr[j][h][1] = v.y; vr[j][h][2] = v.z; vr[j][h][3] = v.w;
-                } else {
-                    const u2 v = *reinterpret_cast<const u2*>(src);
-                    vr[j][h][0] = v.x; vr[j][h][1] = v.y;
+                for (int st = 0; st < KS; st++) kr[h][st] = *reinterpret_cast<const u4*>(src + 32 * st);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const T* src = v_row((j & 4) * 4 + 4 * lg + (j & 3));
+#pragma unroll
+                for (int h = 0; h < NH; h++) {
+                    if constexpr (VE == 8) {
+                        const u4 v = *reinterpret_cast<const u4*>(src + 128 * h);
+                        vr[j][h][0] = v.x; vr[j][h][1] = v.y; vr[j][h][2] = v.z; vr[j][h][3] = v.w;
+                    } else {
+                        const u2 v = *reinterpret_cast<const u2*>(src);
+                        vr[j][h][0] = v.x; vr[j][h][1] = v.y;
+                    }
                 }
             }
+        };
+        if (by_tile) {
+            const long long at = uniform(off);  // of the tile's first key, lane 0's
+            const int most = last - key0;
+            loads([&](int k) { return kp + at + (uint32_t)(min(k, most) * ts + 8 * lg); },
+                  [&](int k) { return vp + at + (uint32_t)(min(k, most) * ts + VE * li); });
+        } else {
+            loads([&](int k) { return kp + __shfl(off, k, 64) + 8 * lg; },
+                  [&](int k) { return vp + __shfl(off, k, 64) + VE * li; });
         }
+        __builtin_amdgcn_sched_barrier(0);  // all loads on their way before the first product waits
+        if (D == 256) read_q();
         f4 s[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -476,10 +515,9 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
     // ---- the wavefronts join in LDS
     l_part += __shfl_xor(l_part, 16, 64);
     l_part += __shfl_xor(l_part, 32, 64);
-    __syncthreads();  // queries read
     if (lg == 0) {
-        s_m[wv][li] = m_ref;
-        s_l[wv][li] = l_part;
+        lds.m[wv][li] = m_ref;
+        lds.l[wv][li] = l_part;
     }
 #pragma unroll
     for (int h = 0; h < NH; h++)
@@ -490,21 +528,20 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
                 *reinterpret_cast<f4*>(&lds.acc[wv][li][VE * 16 * h + VE * (4 * lg + r) + e]) =
                     f4{acc[h][e][r], acc[h][e + 1][r], acc[h][e + 2][r], acc[h][e + 3][r]};
     __syncthreads();
-    float* ws = static_cast<float*>(a.r.ws);
     const bool direct = it.n_split == 1;
     const int part = it.part + it.split * a.p.H_kv;
     for (int i = tid; i < rows * (D / 4); i += 64 * NW) {
         const int row = i / (D / 4), c = (i % (D / 4)) * 4;
-        float m = s_m[0][row];
+        float m = lds.m[0][row];
 #pragma unroll
-        for (int w = 1; w < NW; w++) m = fmaxf(m, s_m[w][row]);
+        for (int w = 1; w < NW; w++) m = fmaxf(m, lds.m[w][row]);
         f4 o = {0.f, 0.f, 0.f, 0.f};
         float l = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float f = __builtin_amdgcn_exp2f(s_m[w][row] - m);
+            const float f = __builtin_amdgcn_exp2f(lds.m[w][row] - m);
             o += *reinterpret_cast<const f4*>(&lds.acc[w][row][c]) * f;
-            l += s_l[w][row] * f;
+            l += lds.l[w][row] * f;
         }
         if (direct) {
             const int r = r0 + row, tok = a.by_rep.div(r), hq = it.head * a.n_rep + r - tok * a.n_rep;
@@ -520,39 +557,31 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
             *reinterpret_cast<u2e*>((T*)a.r.out + (it.row0 + tok) * a.r.out_token + hq * a.r.out_head + c) =
                 u2e{pack<T>(o[0], o[1]), pack<T>(o[2], o[3])};
         } else {
-            *reinterpret_cast<f4*>(part_acc(ws, pt, D, part) + row * D + c) = o;
-            if (c == 0) part_ml(ws, pt, D, part)[row] = float2{m, l};
+            *reinterpret_cast<f4*>(part_acc(a, pt, D, part) + row * D + c) = o;
+            if (c == 0) part_ml(a, pt, D, part)[row] = float2{m, l};
         }
     }
 }
 
-// The splits of a row: W wavefronts sum every W-th and meet in LDS.
-template <typename T, int D, int W>
-__global__ __launch_bounds__(256) void attn_stream_join_kernel(AttnArgs a, Part pt) {
-    constexpr int E = D / 64, RB = 4 / W;  // dims a lane, rows a block
+// The splits of row `row` of an item: a block's JW wavefronts sum every JW-th
+// and meet in LDS, each with eight splits and their maxima in flight.
+template <typename T, int D, int JW>
+__device__ __forceinline__ void stream_join(const AttnArgs& a, const Part& pt, const Item& it, int row) {
+    constexpr int E = D / 64;  // dims a lane
     typedef float fe __attribute__((ext_vector_type(E)));
-    __shared__ float s_o[W > 1 ? W : 1][D];
-    __shared__ float2 s_ml[W];
-    const Schedule sc = schedule<false>(a, pt, true);
-    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, h_kv = a.p.H_kv;
-    for (int x = blockIdx.x; x < sc.total * (16 / RB); x += gridDim.x) {
-    const Item it = item_of(a, pt, sc, x / (16 / RB), true);
-    const int row = x % (16 / RB) * RB + wv / W, r = it.qt * 16 + row;
-    if (r >= it.n_q * a.n_rep) continue;  // (W > 1: of the whole block)
-    if (W > 1) __syncthreads();           // the last row's sums are read
-    float* ws = static_cast<float*>(a.r.ws);
-    const int tok = a.by_rep.div(r), hq = it.head * a.n_rep + r - tok * a.n_rep;
+    __shared__ float s_o[JW][D];
+    __shared__ float2 s_ml[JW];
+    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, h_kv = a.p.H_kv, r = it.qt * 16 + row;
     fe o = {};
     float m = M_NONE, l = 0.0f;
-    // eight splits in flight, their maxima with them
-    for (int i0 = wv % W; i0 < it.n_split; i0 += 8 * W) {
+    for (int i0 = wv; i0 < it.n_split; i0 += 8 * JW) {
         float2 ml[8];
         fe v[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const int i = min(i0 + j * W, it.n_split - 1);
-            ml[j] = part_ml(ws, pt, D, it.part + i * h_kv)[row];
-            v[j] = *reinterpret_cast<const fe*>(part_acc(ws, pt, D, it.part + i * h_kv) + row * D + E * lane);
+            const int i = min(i0 + JW * j, it.n_split - 1);
+            ml[j] = part_ml(a, pt, D, it.part + i * h_kv)[row];
+            v[j] = *reinterpret_cast<const fe*>(part_acc(a, pt, D, it.part + i * h_kv) + row * D + E * lane);
         }
         float top = m;
 #pragma unroll
@@ -563,35 +592,35 @@ __global__ __launch_bounds__(256) void attn_stream_join_kernel(AttnArgs a, Part 
         o *= f0;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            if (i0 + j * W >= it.n_split) break;
+            if (i0 + JW * j >= it.n_split) break;
             const float f = __builtin_amdgcn_exp2f(ml[j].x - m);
             l += ml[j].y * f;
             o += v[j] * f;
         }
     }
-    if constexpr (W > 1) {
+    __syncthreads();  // the last row's sums are read
 #pragma unroll
-        for (int e = 0; e < E; e++) s_o[wv][E * lane + e] = o[e];
-        if (lane == 0) s_ml[wv] = float2{m, l};
-        __syncthreads();
-        if (wv > 0) continue;
-        m = fmaxf(fmaxf(s_ml[0].x, s_ml[1].x), fmaxf(s_ml[2].x, s_ml[3].x));
-        l = 0.0f;
-        o = fe{};
+    for (int e = 0; e < E; e++) s_o[wv][E * lane + e] = o[e];
+    if (lane == 0) s_ml[wv] = float2{m, l};
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c >= D) return;
+    m = s_ml[0].x;
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            const float f = __builtin_amdgcn_exp2f(s_ml[w].x - m);
-            l += s_ml[w].y * f;
+    for (int w = 1; w < JW; w++) m = fmaxf(m, s_ml[w].x);
+    float x = 0.0f;
+    l = 0.0f;
 #pragma unroll
-            for (int e = 0; e < E; e++) o[e] += s_o[w][E * lane + e] * f;
-        }
+    for (int w = 0; w < JW; w++) {
+        const float f = __builtin_amdgcn_exp2f(s_ml[w].x - m);
+        l += s_ml[w].y * f;
+        x += s_o[w][c] * f;
     }
-    const float inv = visible(a, it, r) > 0 ? 1.0f / l : 0.0f;
-    const T* gate = (const T*)a.r.gate + (it.row0 + tok) * a.r.gate_token + hq * a.r.gate_head + E * lane;
-    T* out = (T*)a.r.out + (it.row0 + tok) * a.r.out_token + hq * a.r.out_head + E * lane;
-#pragma unroll
-    for (int e = 0; e < E; e++) out[e] = (T)(o[e] * inv * (a.r.gate ? sigmoid(gate[e]) : 1.0f));
-    }
+    const int tok = a.by_rep.div(r), hq = it.head * a.n_rep + r - tok * a.n_rep;
+    x *= visible(a, it, r) > 0 ? 1.0f / l : 0.0f;
+    if (a.r.gate)
+        x *= sigmoid(((const T*)a.r.gate)[(it.row0 + tok) * a.r.gate_token + hq * a.r.gate_head + c]);
+    ((T*)a.r.out)[(it.row0 + tok) * a.r.out_token + hq * a.r.out_head + c] = (T)x;
 }
 
 // ------------------------------------------------------------ many rows
@@ -605,10 +634,6 @@ __device__ __forceinline__ void load_lds16(const void* g, uint32_t to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g),
                  "s"(__builtin_amdgcn_readfirstlane(to))
                  : "memory");
-}
-__device__ __forceinline__ long long uniform(long long x) {
-    const int lo = __builtin_amdgcn_readfirstlane((int)x), hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
-    return ((long long)hi << 32) | (uint32_t)lo;
 }
 // The same from a uniform address and a lane's bytes.
 __device__ __forceinline__ void load_lds16(const void* g, uint32_t bytes, uint32_t to) {
@@ -627,12 +652,6 @@ __device__ __forceinline__ u2 read_tr(const char* p) {
 
 constexpr int TAB = 1024;  // pages whose byte offsets are in LDS (-1: not a page)
 
-// x, of which the compiler knows nothing: what follows from it is computed where
-// it is used, and not kept in registers that there are not.
-__device__ __forceinline__ int opaque(int x) {
-    asm("" : "+v"(x));
-    return x;
-}
 // The lane, without a register that holds it until then.
 __device__ __forceinline__ int lane_again() {
     int l;
@@ -665,29 +684,26 @@ __device__ __forceinline__ void store_row4(const AttnArgs& a, const Item& it, in
 // 32) + i % 4, which is how V is read, transposed on its way out of LDS.
 // 16-byte pieces of a row are permuted (K: piece ^ key, V: piece ^ 4 key) so
 // that the lanes of a read meet all banks.
-template <typename T, int D, int KG>
-__global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) {
+template <typename T, int D, int KG, int NW>
+__device__ __forceinline__ void tile_item(const AttnArgs& a, const Part& pt, const Item& it, char* lds) {
     constexpr int NS = D / 16, ND = D / 32;  // K steps of a score, dim tiles
     constexpr int ROW = 2 * D, SLOT = 64 * ROW;  // bytes
-    constexpr int CH = D / 8, KPI = 64 / CH, NL = 8 / KPI;  // pieces a row, keys a load, loads of 8 keys
+    constexpr int CH = D / 8, KPI = 64 / CH;  // pieces a row, keys a load
+    constexpr int WK = 64 / NW, NL = WK / KPI;     // keys a wavefront loads, its loads
     constexpr int AHEAD = D == 64 ? 4 : D == 128 ? 6 : 3;
     // Q operands that stay in LDS: a register file holds 128 of O, 64 of Q, 16
     // scores and 16 of operands, and a few too few for what goes with them.
     constexpr int QL = D == 256 ? 2 : 0;
     typedef typename V<T>::x8 x8;
-    extern __shared__ __align__(1024) char lds[];
     char* const ks = lds;
     char* const vs = lds + 2 * SLOT;
     long long* const tab = reinterpret_cast<long long*>(lds + 4 * SLOT);
     __shared__ int s_bad;
     __shared__ float2 s_ml[2][4][32];
-    const Schedule sc = schedule<true>(a, pt, false);
-    if ((int)blockIdx.x >= sc.total) return;
-    const Item it = item_of(a, pt, sc, blockIdx.x, false);
     const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int ln = lane & 31, hh = lane >> 5;
     const int rg = KG == 1 ? wv : wv & 3, kg = KG == 1 ? 0 : wv >> 2;
-    constexpr int BR = 256 / KG;
+    constexpr int BR = 32 * NW / KG;
     const int n_rows = it.n_q * a.n_rep;
     // (a lane of no row is the last row again and stores nothing)
     const int r_in = min(it.qt * BR + rg * 32 + ln, n_rows - 1);
@@ -701,7 +717,7 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
     auto fill = [&](int u) __attribute__((always_inline)) {
         w0 = a.by_page.div(u * 64);
         const int n = min(TAB, a.by_page.div(vis_hi - 1) + 1 - w0);
-        for (int i = wv * 64 + lane_again(); i < n; i += 512) {
+        for (int i = wv * 64 + lane_again(); i < n; i += 64 * NW) {
             const int e = a.r.table[(size_t)it.seq * a.r.table_ld + w0 + i];
             const bool bad = (unsigned)e >= (unsigned)a.p.n_pages;
             tab[i] = bad ? -1 : 2 * (e * a.p.page_stride);
@@ -720,27 +736,27 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
     const char* const kh = (const char*)a.p.k + 2 * (it.head * a.p.head_stride);
     const char* const vh = (const char*)a.p.v + 2 * (it.head * a.p.head_stride);
     const int last = vis_hi - 1;
-    const bool by_group = a.p.page_size % 8 == 0 && a.p.token_stride * a.p.page_size < 1 << 28;
+    const bool by_group = a.p.page_size % WK == 0 && a.p.token_stride * a.p.page_size < 1 << 28;
     auto stage = [&](int u) __attribute__((always_inline)) {
         const int l = lane_again(), lk = l / CH, p = l % CH;
         const uint32_t to = ((u - u_lo) & 1) * SLOT + wv * NL * 1024;
         auto piece_k = [&](int key) { return (p ^ (D == 64 ? (key >> 1) & 7 : key & 15)) << 4; };
         auto piece_v = [&](int key) { return (p ^ (D == 64 ? (key & 2) << 1 : (key & 3) << 2)) << 4; };
         if (by_group) {
-            const int t = min(u * 64 + wv * 8, last & ~7), pg = a.by_page.div(t);
+            const int t = min(u * 64 + wv * WK, last & ~(WK - 1)), pg = a.by_page.div(t);
             const int ts2 = 2 * (int)a.p.token_stride;
             const long long at = uniform(max(uniform(tab[pg - w0]), 0ll) + (t - pg * a.p.page_size) * ts2);
             const int most = last - t;
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                const int row = i * KPI + lk, key = wv * 8 + row, off = min(row, most) * ts2;
+                const int row = i * KPI + lk, key = wv * WK + row, off = min(row, most) * ts2;
                 load_lds16(kh + at, off + piece_k(key), lds_addr(ks) + to + i * 1024);
                 load_lds16(vh + at, off + piece_v(key), lds_addr(vs) + to + i * 1024);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                const int key = wv * 8 + i * KPI + lk, t = min(u * 64 + key, last), pg = a.by_page.div(t);
+                const int key = wv * WK + i * KPI + lk, t = min(u * 64 + key, last), pg = a.by_page.div(t);
                 const long long off = max(tab[pg - w0], 0ll) + 2 * ((t - pg * a.p.page_size) * a.p.token_stride);
                 load_lds16(kh + off + piece_k(key), lds_addr(ks) + to + i * 1024);
                 load_lds16(vh + off + piece_v(key), lds_addr(vs) + to + i * 1024);
@@ -790,12 +806,12 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
                 fill(u);
                 __syncthreads();
             }
-            if (wv >= 4) stage(u + 1);
+            if (NW == 4 || wv >= 4) stage(u + 1);
         }
     };
     auto keys = [&](int u, auto masked) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
-        bool staged = wv >= 4 || u + 1 >= u_hi;
+        bool staged = NW == 4 || wv >= 4 || u + 1 >= u_hi;
 #pragma unroll 1
         for (int sub = kg; sub < 2; sub += KG) {
             const int key0 = u * 64 + 32 * sub;
@@ -911,7 +927,7 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
         }
         if (MASKED && !staged) stage(u + 1);
     };
-    if (wv >= 4) __builtin_amdgcn_s_setprio(1);
+    if (NW == 8 && wv >= 4) __builtin_amdgcn_s_setprio(1);
     // units that every row sees whole, then the others; all from the first entry
     // outside the cache on
     const int u_mid = min(u_hi, visible(a, it, it.qt * BR) >> 6);
@@ -935,15 +951,14 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
     // res[i][4 q + c].  (Code that runs once a block costs more to fetch than to
     // run: the halves are a loop, and a row's place is computed by one lane.)
     auto leave_part = [&](const f16v(&res)[HD], int half) __attribute__((always_inline)) {
-        float* ws = static_cast<float*>(a.r.ws);
-        const int part = it.part + it.split * a.p.H_kv;
-        f4* const x = reinterpret_cast<f4*>(part_acc(ws, pt, D, part)) + (rg * ND + half * HD) * (4 * 64) + el;
+            const int part = it.part + it.split * a.p.H_kv;
+        f4* const x = reinterpret_cast<f4*>(part_acc(a, pt, D, part)) + (rg * ND + half * HD) * (4 * 64) + el;
 #pragma unroll
         for (int i = 0; i < HD; i++)
 #pragma unroll
             for (int q = 0; q < 4; q++)
                 x[(i * 4 + q) * 64] = f4{res[i][4 * q], res[i][4 * q + 1], res[i][4 * q + 2], res[i][4 * q + 3]};
-        if (ehh == 0 && half == 0) part_ml(ws, pt, D, part)[rg * 32 + eln] = float2{m_ref, l_row};
+        if (ehh == 0 && half == 0) part_ml(a, pt, D, part)[rg * 32 + eln] = float2{m_ref, l_row};
     };
     // Outputs go through LDS, so that a lane stores 16 bytes next to its
     // neighbours': lane el takes 8-dim group el % GN of row el / GN of RI at once.
@@ -1040,19 +1055,13 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(AttnArgs a, Part pt) 
     }
 }
 
-// The splits of 32 rows: a wavefront 8 dims of them, a block 32.
+// The splits of 32 rows (group rg of the tile), dims 8 piece and on: a wavefront.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_tile_join_kernel(AttnArgs a, Part pt) {
+__device__ __forceinline__ void tile_join(const AttnArgs& a, const Part& pt, const Item& it, int rg, int piece) {
     constexpr int ND = D / 32;
-    const int groups = pt.rows / 32;
-    const Schedule sc = schedule<false>(a, pt, true);
-    const int q = threadIdx.x >> 6, lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5;
-    for (int x = blockIdx.x; x < sc.total * groups * ND; x += gridDim.x) {
-    const Item it = item_of(a, pt, sc, x / (groups * ND), true);
-    const int rg = x / ND % groups, i = x % ND;
+    const int i = piece >> 2, q = piece & 3, lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5;
     const int r = it.qt * pt.rows + rg * 32 + ln, h_kv = a.p.H_kv;
-    if (r >= it.n_q * a.n_rep) continue;
-    float* ws = static_cast<float*>(a.r.ws);
+    if (r >= it.n_q * a.n_rep) return;
     f4 o = {};
     float m = M_NONE, l = 0.0f;
     for (int s0 = 0; s0 < it.n_split; s0 += 8) {
@@ -1061,8 +1070,8 @@ __global__ __launch_bounds__(256) void attn_tile_join_kernel(AttnArgs a, Part pt
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int s = min(s0 + j, it.n_split - 1);
-            ml[j] = part_ml(ws, pt, D, it.part + s * h_kv)[rg * 32 + ln];
-            v[j] = reinterpret_cast<const f4*>(part_acc(ws, pt, D, it.part + s * h_kv))[((rg * ND + i) * 4 + q) * 64 + lane];
+            ml[j] = part_ml(a, pt, D, it.part + s * h_kv)[rg * 32 + ln];
+            v[j] = reinterpret_cast<const f4*>(part_acc(a, pt, D, it.part + s * h_kv))[((rg * ND + i) * 4 + q) * 64 + lane];
         }
         float top = m;
 #pragma unroll
@@ -1081,81 +1090,120 @@ __global__ __launch_bounds__(256) void attn_tile_join_kernel(AttnArgs a, Part pt
     }
     const float inv = visible(a, it, r) > 0 ? 1.0f / l : 0.0f;
     store_row4<T>(a, it, r, 32 * i + 8 * q + 4 * hh, o * inv);
+}
+
+// ------------------------------------------------------------ the launches
+extern __shared__ __align__(1024) char dyn_lds[];
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnArgs a, Part ps) {
+    const Schedule sc = schedule<false>(a, ps, false);
+    if ((int)blockIdx.x >= sc.total) return;
+    stream_item<T, D, STREAM_WAVES>(a, ps, item_of(a, ps, sc, blockIdx.x, false), dyn_lds);
+}
+
+// Tiles of the sequences of many rows, then those of few: a continuous batch's
+// decoding sequences run beside its chunks (two launches one after the other
+// and two joins took 105 us of a batch of 24).
+template <typename T, int D, int KG, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_tile_kernel(AttnArgs a, Part pl, Part ps) {
+    const Schedule sl = schedule<true>(a, pl, false);
+    const int x = blockIdx.x - sl.total;
+    if (x < 0) {
+        tile_item<T, D, KG, NW>(a, pl, item_of(a, pl, sl, blockIdx.x, false), dyn_lds);
+        return;
     }
+    const Schedule sc = schedule<false>(a, ps, false);
+    if (x < sc.total) stream_item<T, D, NW>(a, ps, item_of(a, ps, sc, x, false), dyn_lds);
+}
+
+// row_step: rows of a row tile of 16 that there should be (others follow).
+template <typename T, int D, int JW>
+__global__ __launch_bounds__(64 * JW) void attn_join_kernel(AttnArgs a, Part pl, Part ps, int row_step) {
+    const Schedule sc = schedule<false>(a, ps, true);
+    for (int x = blockIdx.x; x < sc.total * row_step; x += gridDim.x) {
+        const int k = (int)((uint32_t)x / (uint32_t)row_step);
+        const Item it = item_of(a, ps, sc, k, true);
+        const int rows = min(16, it.n_q * a.n_rep - it.qt * 16);
+        for (int row = x - k * row_step; row < rows; row += row_step) stream_join<T, D, JW>(a, ps, it, row);
+    }
+    if (pl.slots == 0) return;
+    const Schedule sl = schedule<false>(a, pl, true);
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = pl.rows / 32 * (D / 8);
+    for (int x = blockIdx.x * JW + wv; x < sl.total * per; x += gridDim.x * JW)
+        tile_join<T, D>(a, pl, item_of(a, pl, sl, x / per, true), x % per / (D / 8), x % (D / 8));
 }
 
 // What a call of these sizes launches.
 struct Plan {
-    bool stream, tile;
-    Part ps, pl;
-    int stream_blocks, stream_joins, tile_blocks, tile_joins, kg;
+    bool tile;  // sequences of many rows there may be
+    Part pl, ps;
+    int blocks, waves, kg, joins, join_waves, row_step;
 };
-// Blocks for up to `items` items: one round of slots while they may be few,
-// else cost / u more than items (schedule), u at least half a slot's share.
-int blocks_for(long long items, int slots) {
-    return (int)(items + slots);
-}
-Plan plan_of(int n_tok, int n_seq, int H_q, int H_kv, int max_q) {
+size_t part_floats(const Part& pt, int d) { return (size_t)2 * pt.slots * pt.rows * (d + 2); }
+
+// max_q only chooses between the two launches: either serves every sequence.
+Plan plan_of(int n_tok, int n_seq, int H_q, int H_kv, int d, int max_q) {
     const int n_rep = H_q / H_kv, seqs = std::min(n_tok, n_seq);
     const long long rows = (long long)n_tok * n_rep;
     Plan p{};
-    p.stream = true;  // there may be short sequences whatever max_q says
     p.tile = (long long)max_q * n_rep > SMALL_ROWS;
-    p.ps = Part{16, STREAM_UNIT, STREAM_SLOTS, p.tile ? SERVE_SMALL : SERVE_ALL};
-    // row tiles there may be: those served hold 16 rows or, served all, n_tok's
-    const long long most = p.tile ? (long long)seqs * H_kv : (rows / 16 + seqs) * H_kv;
-    p.stream_blocks = blocks_for(most, STREAM_SLOTS);
-    p.stream_joins = (int)std::min<long long>(STREAM_SLOTS, most);
-    p.kg = rows / 256 * H_kv >= TILE_SLOTS ? 1 : 2;
-    const int br = 256 / p.kg;
-    p.pl = Part{br, TILE_UNIT, TILE_SLOTS, SERVE_LARGE};
-    const long long tiles = (rows / br + seqs) * H_kv;
-    p.tile_blocks = blocks_for(tiles, TILE_SLOTS);
-    p.tile_joins = (int)std::min<long long>(TILE_SLOTS, tiles);
+    if (p.tile) {
+        // 256 dims fill LDS with one block's keys and values: 8 wavefronts on 256
+        // rows or, where those tiles would be fewer than the CUs, 128.  Else two
+        // blocks of 4 on 128 rows, one of which starts or ends while the other works.
+        p.waves = d == 256 ? 8 : 4;
+        p.kg = d == 256 && rows / 256 * H_kv < 256 ? 2 : 1;
+        const int slots = d == 256 ? 256 : 512;
+        p.pl = Part{32 * p.waves / p.kg, TILE_UNIT, slots, SERVE_LARGE, 0};
+        p.ps = Part{16, 32 * p.waves, slots, SERVE_SMALL, part_floats(p.pl, d)};
+    } else {
+        p.waves = STREAM_WAVES;
+        p.ps = Part{16, 32 * STREAM_WAVES, STREAM_SLOTS, SERVE_ALL, 0};
+    }
+    // row tiles there may be, and blocks: schedule makes at most `slots` more
+    const long long large = p.tile ? (rows / p.pl.rows + seqs) * H_kv : 0;
+    const long long small = p.tile ? (long long)seqs * H_kv : (rows / 16 + seqs) * H_kv;
+    p.blocks = (int)(large + p.pl.slots + small + p.ps.slots);
+    p.row_step = (int)std::min<long long>(16, (long long)max_q * n_rep);
+    const long long items = std::min<long long>(p.ps.slots, small) * p.row_step;
+    // few rows may have many splits
+    p.join_waves = !p.tile && items <= 64 ? 16 : 4;
+    const long long pieces = std::min<long long>(p.pl.slots, large) * (p.pl.rows / 32) * (d / 8);
+    p.joins = (int)std::min<long long>(items + (pieces + p.join_waves - 1) / p.join_waves, 2048);
     return p;
 }
-size_t part_bytes(const Part& pt, int d) {
-    return (size_t)2 * pt.slots * pt.rows * (d * sizeof(float) + sizeof(float2));
-}
 
-template <typename T, int D, int KG>
-hipError_t launch_tile(const AttnArgs& a, const Plan& p, hipStream_t st) {
-    constexpr int bytes = 4 * 64 * 2 * D + TAB * (int)sizeof(long long) + (D == 256 ? 8 * 2 * 1024 : 0);
-    const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(attn_tile_kernel<T, D, KG>), bytes);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((attn_tile_kernel<T, D, KG>), dim3(p.tile_blocks), dim3(512), bytes, st, a, p.pl);
-    hipLaunchKernelGGL((attn_tile_join_kernel<T, D>), dim3(std::min(2048, p.tile_joins * (p.pl.rows / 32) * (D / 32))),
-                       dim3(256), 0, st, a, p.pl);
-    return hipGetLastError();
-}
+// LDS of stream_item.
+constexpr int stream_bytes(int waves, int d) { return waves * 16 * (d + 6) * (int)sizeof(float) + 16 * (d + 8) * 2; }
 
 template <typename T, int D>
 hipError_t launch(const AttnArgs& a, hipStream_t st) {
-    const Plan p = plan_of(a.r.n_tok, a.r.n_seq, a.r.H_q, a.p.H_kv, a.r.max_q);
+    const Plan p = plan_of(a.r.n_tok, a.r.n_seq, a.r.H_q, a.p.H_kv, D, a.r.max_q);
     if (p.tile) {
-        const hipError_t e = p.kg == 1 ? launch_tile<T, D, 1>(a, p, st) : launch_tile<T, D, 2>(a, p, st);
+        constexpr int NW = D == 256 ? 8 : 4;
+        constexpr int bytes = 4 * 64 * 2 * D + TAB * (int)sizeof(long long) + (D == 256 ? 8 * 2 * 1024 : 0);
+        static_assert(bytes >= stream_bytes(NW, D), "the stream's wavefronts join there");
+        auto* const k = D < 256 || p.kg == 1 ? attn_tile_kernel<T, D, 1, NW> : attn_tile_kernel<T, D, D == 256 ? 2 : 1, NW>;
+        const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(k), bytes);
         if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(k, dim3(p.blocks), dim3(64 * NW), bytes, st, a, p.pl, p.ps);
+    } else {
+        constexpr int bytes = stream_bytes(STREAM_WAVES, D);
+        const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(attn_stream_kernel<T, D>), bytes);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((attn_stream_kernel<T, D>), dim3(p.blocks), dim3(64 * STREAM_WAVES), bytes, st, a, p.ps);
     }
-    if (p.stream) {
-        hipLaunchKernelGGL((attn_stream_kernel<T, D>), dim3(p.stream_blocks), dim3(64 * STREAM_WAVES), 0,
-                           st, a, p.ps);
-        // few rows of many splits: a block a row (one sequence of 512 tokens and 24 / 4
-        // heads ...), else a wavefront a row
-        if (p.stream_joins <= 32)
-            hipLaunchKernelGGL((attn_stream_join_kernel<T, D, 4>), dim3(p.stream_joins * 16), dim3(256), 0, st,
-                               a, p.ps);
-        else
-            hipLaunchKernelGGL((attn_stream_join_kernel<T, D, 1>), dim3(std::min(2048, p.stream_joins * 4)), dim3(256), 0, st, a,
-                               p.ps);
-    }
+    auto* const join = p.join_waves == 16 ? attn_join_kernel<T, D, 16> : attn_join_kernel<T, D, 4>;
+    hipLaunchKernelGGL(join, dim3(p.joins), dim3(64 * p.join_waves), 0, st, a, p.pl, p.ps, p.row_step);
     return hipGetLastError();
 }
 
 }  // namespace
 
 size_t attn_ws_bytes(int n_tok, int n_seq, int H_q, int H_kv, int head_dim, int max_q) {
-    const Plan p = plan_of(n_tok, n_seq, H_q, H_kv, max_q);
-    return std::max(part_bytes(p.ps, head_dim), part_bytes(p.pl, head_dim));
+    const Plan p = plan_of(n_tok, n_seq, H_q, H_kv, head_dim, max_q);
+    return (part_floats(p.pl, head_dim) + part_floats(p.ps, head_dim)) * sizeof(float);
 }
 
 hipError_t launch_attn(const AttnArgs& a, hipStream_t st) {

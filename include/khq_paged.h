@@ -125,7 +125,10 @@ typedef struct khq_attn_rows {
 /* Attention of the new tokens over the pages: row i of sequence s (of n_q
  * rows) sees the sequence's first seq_kv[s] - n_q + i + 1 tokens, so a single
  * row sees them all; query head h reads KV head h / (H_q / H_kv).  A row that
- * sees none is 0.  Rows of no sequence (a padded batch) are left as they were.
+ * sees none is 0.  Rows of no sequence (a padded batch) are left as they were; a
+ * sequence that starts or ends outside the batch has those inside, or none if it
+ * starts below 0 or ends before it starts; what rows of two sequences hold is
+ * not said.
  * A table entry outside [0, n_pages) among the tokens a row's sequence holds
  * makes rows that see it NaN; nothing outside the cache is read.
  *
