@@ -35,12 +35,14 @@ ROWS_STRUCT = struct.Struct("=10Q12qdf8i4x")
 ATTN_STRUCT = struct.Struct("=7QQ6qf5i")
 
 MAX_SEQ = 4096  # KHQ_PAGED_MAX_SEQ
+_INT32 = torch.int32
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _HEAD_DIMS = (64, 128, 256)
 
 _paged = None
 # the raw handle of a device's current stream, where this torch has it
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def lib() -> ctypes.CDLL:
@@ -65,11 +67,16 @@ def _call(name: str, *args, check: bool = True) -> int:
     return rc
 
 
+# A step's calls are as long as their checks on the host: each check reads an
+# argument once and in one condition, and only its failure asks what was wrong.
 def _i32(t, n: int, name: str, device: int) -> int:
     """Pointer of a contiguous int32 tensor of n elements on this device."""
-    if (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == device
-            and t.numel() == n and t.is_contiguous()):
-        return t.data_ptr()
+    try:
+        if (t.dtype is _INT32 and t.numel() == n and t.get_device() == device
+                and t.is_contiguous()):
+            return t.data_ptr()
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
     if t.dtype != torch.int32:
@@ -96,12 +103,14 @@ def _table(t, n_seq, device: int):
 def _heads(t, shape, dtype, name: str, device: int):
     """(pointer, token stride, head stride) of a [tokens][heads][dims] tensor whose
     dims are dense; tokens and heads may be strided."""
-    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device
-            and t.shape == shape):
-        token, head, dim = t.stride()
-        if dim == 1:
-            return t.data_ptr(), token, head
-        raise ValueError(f"{name}: its last dim must be dense")
+    try:
+        if t.shape == shape and t.dtype is dtype and t.get_device() == device:
+            token, head, dim = t.stride()
+            if dim == 1:
+                return t.data_ptr(), token, head
+            raise ValueError(f"{name}: its last dim must be dense")
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
     if t.dtype != dtype:
@@ -129,12 +138,12 @@ def _device(t, name: str) -> int:
     """Index of the current device, the tensor's."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
-    if not t.is_cuda:
-        raise ValueError(f"{name}: must be a device tensor")
     device = t.get_device()
-    if device != torch.cuda.current_device():
+    if device < 0:
+        raise ValueError(f"{name}: must be a device tensor")
+    if device != _current_device():
         raise ValueError(f"{name}: on {t.device}, but the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
+                         f"cuda:{_current_device()}")
     return device
 
 
@@ -153,15 +162,16 @@ def _pages(k, v, device: int):
             raise TypeError(f"{name}: expected a torch.Tensor")
         if t.get_device() != device:
             raise ValueError(f"{name}: on {t.device}, expected cuda:{device}")
-    dtype = _DTYPES.get(k.dtype)
-    if dtype is None:
-        raise TypeError(f"k_pages: dtype {k.dtype}, expected float16 or bfloat16")
+    dtype = k.dtype
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"k_pages: dtype {dtype}, expected float16 or bfloat16")
     shape = k.shape
     if len(shape) != 4 or shape[3] not in _HEAD_DIMS or 0 in shape:
         raise ValueError(f"k_pages: shape {tuple(shape)}, expected "
                          "[pages][page_size][heads][64, 128 or 256]")
     strides = k.stride()
-    if v.shape != shape or v.stride() != strides or v.dtype != k.dtype:
+    if v.shape != shape or v.stride() != strides or v.dtype is not dtype:
         raise ValueError("v_pages: shape, strides and dtype must be those of k_pages")
     page, token, head, dim = strides
     kp, vp = k.data_ptr(), v.data_ptr()
@@ -171,7 +181,7 @@ def _pages(k, v, device: int):
     n_pages, page_size, h_kv, d = shape
     if n_pages * page_size >= 1 << 31:
         raise ValueError("k_pages: 2^31 slots or more")
-    return PAGES_STRUCT.pack(kp, vp, page, token, head, n_pages, page_size, h_kv, d, dtype), shape
+    return PAGES_STRUCT.pack(kp, vp, page, token, head, n_pages, page_size, h_kv, d, code), shape
 
 
 def plan(q_len, kv_len, table, free_pages, state, *, page_size: int, cu_q, seq_kv, kv_out,
