@@ -12,6 +12,7 @@ checked on the host before the launch, which goes to the current HIP stream (or
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import struct
 
@@ -19,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import KhqError, ptr, stream_handle
-from .build import PAGED_LIB_PATH
+from .build import PAGED_CALLS_PATH, PAGED_LIB_PATH
 
 P, I = ctypes.c_void_p, ctypes.c_int
 
@@ -311,6 +312,21 @@ def attn_ws_bytes(n_tok: int, n_seq: int, H_q: int, H_kv: int, head_dim: int, ma
     if n < 0:
         raise KhqError("khq_paged_attn_ws_bytes", n)
     return n
+
+
+def _native(*functions):
+    """The functions behind the checks of khq._paged, which take what is as it should be to
+    the same C entry in a microsecond and leave the rest to them (here 4 to 8 us)."""
+    if _raw_stream is None or not os.path.exists(PAGED_CALLS_PATH):
+        return functions
+    lib()
+    from . import _paged as calls
+
+    calls.init(KhqError, _raw_stream)
+    return [functools.update_wrapper(calls.Call(f), f) for f in functions]
+
+
+plan, qk_norm_rope, attn = _native(plan, qk_norm_rope, attn)
 
 
 class PageTable:
