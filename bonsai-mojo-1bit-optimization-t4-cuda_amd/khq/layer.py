@@ -359,6 +359,29 @@ class NativeKhqLayer:
             raise KhqError("khq_layer_prefill", rc)
         return rc
 
+    def attention_prefill(self, q_gate, k, v, out, scale: float, *, pos: int, q_norm_w=None,
+                          k_norm_w=None, eps: float = 1e-6) -> int:
+        """attention_step for n tokens at once, at positions pos .. pos + n - 1: head RMSNorm
+        and partial RoPE of q_gate's queries f16 [n][H_q][512] and of k f16 [n][H_kv][256] (in
+        place) in one pass, then prefill.  A recorder's dumps are of single tokens: with one
+        attached, use attention_step."""
+        from . import paged
+
+        if getattr(self, "_dump", None) is not None:
+            raise RuntimeError("attention_prefill: a dump recorder is attached")
+        n = q_gate.shape[0]
+        ops._need(q_gate, torch.float16, n * self.H_q * 2 * D, "q_gate")
+        ops._need(k, torch.float16, n * self.H_kv * D, "k")
+        ops._need(v, torch.float16, n * self.H_kv * D, "v")
+        ops._need(out, torch.float16, n * self.H_q * D, "out")
+        q = q_gate.view(n, self.H_q, 2 * D)[..., :D]
+        k = k.view(n, self.H_kv, D)
+        unroped = torch.empty_like(k)
+        paged.qk_norm_rope(q, k, q, pos0=pos, q_weight=q_norm_w, k_weight=k_norm_w, eps=eps,
+                           theta=ROPE_BASE, rotary_dim=64, k_out=k, k_normed=unroped,
+                           round_norm=True)
+        return self.prefill(q_gate, k, v, unroped, out, scale)
+
 
 class KhqRuntime:
     """khq_activate / khq_init: loads a KHQK v2 file and creates the layers
