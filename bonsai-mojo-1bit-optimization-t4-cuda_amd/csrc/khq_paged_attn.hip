@@ -113,6 +113,7 @@ struct Part {
     int rows;   // of a row tile
     int unit;   // keys
     int slots;  // blocks
+    int room;   // of them, what the cost is shared among where items are nearly as many
     Serve serve;
     size_t at;  // of its partial results in the workspace, in floats
 };
@@ -170,11 +171,11 @@ __device__ __forceinline__ T lane63(T v) {
 // those of the longest blocks first; within a sequence, KV heads in turn
 // (blocks go to the XCDs in turn, so a head's row tiles meet its keys in one
 // L2), then splits, then row tiles from the last, which sees most keys, to the
-// first.  A block takes at most u units.  With items fewer than half the slots
+// first.  A block takes at most u units.  With items few beside the slots
 // u = cost / (slots - items): sum of ceil(units / u) <= cost / u + items <=
-// slots, one round of blocks.  With more, twice a slot's share of the cost, and
-// from the slots' own number on once that share: alike items stay whole, one of
-// a long sequence among short ones does not outlast the others.  Partial
+// slots, one round of blocks.  With more, cost / room, and from the slots' own
+// number on cost / slots: alike items stay whole, one of a long sequence among
+// short ones does not outlast the others.  Partial
 // results: at most 2 cost / u <= 2 slots, as an item that is split has more
 // than u units.  (The cost is a float sum, taken a little larger.)
 struct Schedule {
@@ -201,7 +202,7 @@ __device__ __forceinline__ Schedule schedule(const AttnArgs& a, const Part& pt, 
         cost += (float)(sc.one.tiles * h_kv) * (float)sc.one.units;
     }
     const int all = lane63(scan_add(items));
-    const int room = all >= pt.slots ? pt.slots : max(pt.slots - all, pt.slots / 2);
+    const int room = all >= pt.slots ? pt.slots : max(pt.slots - all, pt.room);
     const float share = lane63(scan_add(cost)) * 1.00001f / (float)room;
     sc.u = max(1, (int)fminf(ceilf(share), 1e9f));
     int n_part = 0, longest = 0;
@@ -1155,11 +1156,15 @@ Plan plan_of(int n_tok, int n_seq, int H_q, int H_kv, int d, int max_q) {
         p.waves = d == 256 ? 8 : 4;
         p.kg = d == 256 && rows / 256 * H_kv < 256 ? 2 : 1;
         const int slots = d == 256 ? 256 : 512;
-        p.pl = Part{32 * p.waves / p.kg, TILE_UNIT, slots, SERVE_LARGE, 0};
-        p.ps = Part{16, 32 * p.waves, slots, SERVE_SMALL, part_floats(p.pl, d)};
+        // With a block a CU, a share of half the slots: more blocks cost more than
+        // they level (3 chunks of 363: 43 us, with 3/4 58).  With two, one that ends
+        // early leaves the CU to the other: 3/4 (12 chunks of 41: 43.5 us for 45.3).
+        const int room = d == 256 ? slots / 2 : slots / 4 * 3;
+        p.pl = Part{32 * p.waves / p.kg, TILE_UNIT, slots, room, SERVE_LARGE, 0};
+        p.ps = Part{16, 32 * p.waves, slots, slots / 2, SERVE_SMALL, part_floats(p.pl, d)};
     } else {
         p.waves = STREAM_WAVES;
-        p.ps = Part{16, 32 * STREAM_WAVES, STREAM_SLOTS, SERVE_ALL, 0};
+        p.ps = Part{16, 32 * STREAM_WAVES, STREAM_SLOTS, STREAM_SLOTS / 2, SERVE_ALL, 0};
     }
     // row tiles there may be, and blocks: schedule makes at most `slots` more
     const long long large = p.tile ? (rows / p.pl.rows + seqs) * H_kv : 0;
