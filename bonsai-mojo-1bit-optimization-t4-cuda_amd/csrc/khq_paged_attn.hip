@@ -187,6 +187,9 @@ struct Schedule {
 __device__ __forceinline__ int splits_of(const Schedule& sc, const SeqLen& l) {
     return l.units <= sc.u ? 1 : (int)ceilf((float)l.units / (float)sc.u);
 }
+// (64 lanes' stay in 31 bits: a batch within the sizes has 2^23, but cu_q may
+// name the same rows for many sequences)
+constexpr int MOST_ITEMS = 1 << 24;
 template <bool LONG>
 __device__ __forceinline__ Schedule schedule(const AttnArgs& a, const Part& pt, bool joining) {
     const int lane = threadIdx.x & 63, n_seq = a.r.n_seq, h_kv = a.p.H_kv;
@@ -198,7 +201,7 @@ __device__ __forceinline__ Schedule schedule(const AttnArgs& a, const Part& pt, 
     float cost = 0.0f;
     for (int s = s0; s < s1; s++) {
         sc.one = seq_len(a, pt, s);
-        items += sc.one.tiles * h_kv;
+        items = min(items + sc.one.tiles * h_kv, MOST_ITEMS);
         cost += (float)(sc.one.tiles * h_kv) * (float)sc.one.units;
     }
     const int all = lane63(scan_add(items));
@@ -211,7 +214,7 @@ __device__ __forceinline__ Schedule schedule(const AttnArgs& a, const Part& pt, 
         if (sc.per > 1) sc.one = seq_len(a, pt, s);
         const int n = sc.one.tiles * h_kv, sp = splits_of(sc, sc.one);
         n_part += sp > 1 ? n * sp : 0;
-        sc.n_item += joining ? (sp > 1 ? n : 0) : n * sp;
+        sc.n_item = min(sc.n_item + (joining ? (sp > 1 ? n : 0) : n * sp), MOST_ITEMS);
         if (LONG) longest = (int)((float)sc.one.units / (float)sp);
     }
     sc.at = scan_add(sc.n_item);

@@ -6,6 +6,7 @@
 
 #include <cmath>
 #include <cstring>
+#include <mutex>
 
 #include "khq_paged.h"
 #include "khq_paged_internal.h"
@@ -56,11 +57,15 @@ int khq_qk_norm_rope(const khq_rows* rows, const khq_pages* pages, hipStream_t s
         (r.q && (!r.q_out || r.H_q <= 0)) || (r.k && r.H_kv <= 0) || r.pos0 < 0)
         return -100;
     if (r.rotary_dim < 0 || r.rotary_dim > r.head_dim || r.rotary_dim % 16 != 0 ||
-        (r.rotary_dim > 0 && !(r.theta > 0.0)))
+        (r.rotary_dim > 0 && !(r.theta > 0.0 && std::isfinite(r.theta))))
         return -100;
     if (pages && (!pages_ok(pages) || !r.k || !r.v || !r.slots || pages->H_kv != r.H_kv ||
                   pages->head_dim != r.head_dim || pages->dtype != r.dtype))
         return -100;
+    if (pages && ((pages->n_pages > 1 && pages->page_stride < r.head_dim) ||
+                  (pages->page_size > 1 && pages->token_stride < r.head_dim) ||
+                  (pages->H_kv > 1 && pages->head_stride < r.head_dim)))
+        return -100;  // slots that share memory, as an expanded tensor's do
     if (!pages && r.k && !r.k_out && !r.k_normed) return -100;  // nothing to leave the keys in
     if (r.n == 0) return 0;
     khq::paged::RowsArgs a{};
@@ -84,7 +89,8 @@ int khq_qk_norm_rope(const khq_rows* rows, const khq_pages* pages, hipStream_t s
 
 static bool attn_sizes_ok(int n_tok, int n_seq, int H_q, int H_kv, int head_dim, int max_q) {
     return n_tok >= 0 && n_seq > 0 && n_seq <= KHQ_PAGED_MAX_SEQ && H_q > 0 && H_kv > 0 &&
-           H_q % H_kv == 0 && dim_ok(head_dim) && max_q > 0 && (long long)n_tok * H_q < 0x7fffffffLL;
+           H_q % H_kv == 0 && dim_ok(head_dim) && max_q > 0 && (long long)n_tok * H_q < 1LL << 27 &&
+           (long long)n_seq * H_kv <= 1LL << 21;  // a launch's blocks
 }
 
 long long khq_paged_attn_ws_bytes(int n_tok, int n_seq, int H_q, int H_kv, int head_dim, int max_q) {
@@ -97,7 +103,7 @@ int khq_paged_attn(const khq_attn_rows* rows, const khq_pages* pages, hipStream_
     const khq_attn_rows& r = *rows;
     if (!attn_sizes_ok(r.n_tok, r.n_seq, r.H_q, pages->H_kv, pages->head_dim, r.max_q) || !r.q ||
         !r.out || !r.cu_q || !r.seq_kv || !r.table || r.table_ld <= 0 ||
-        (long long)r.table_ld * pages->page_size > 0x7fffffffLL)
+        (long long)r.table_ld * pages->page_size > 0x7fffffffLL || !std::isfinite(r.scale))
         return -100;
     if (r.n_tok == 0) return 0;
     khq::paged::AttnArgs a{};
@@ -111,12 +117,16 @@ int khq_paged_attn(const khq_attn_rows* rows, const khq_pages* pages, hipStream_
                                                   pages->head_dim, r.max_q);
     if (r.ws) {
         if (r.ws_bytes < need || (reinterpret_cast<uintptr_t>(r.ws) & 15)) return -101;
-    } else if (need > 0) {
-        float* ws = nullptr;
-        const hipError_t e = khq::shared_workspace(need, stream, &ws);
-        if (e != hipSuccess) return rc_of(e);
-        a.r.ws = ws;
+        return rc_of(khq::paged::launch_attn(a, stream));
     }
+    // One caller at a time takes the shared workspace and launches: the next one's
+    // stream waits for these launches, and its growing it does not come between.
+    static std::mutex launching;
+    std::lock_guard<std::mutex> lock(launching);
+    float* ws = nullptr;
+    const hipError_t e = khq::shared_workspace(need, stream, &ws);
+    if (e != hipSuccess) return rc_of(e);
+    a.r.ws = ws;
     return rc_of(khq::paged::launch_attn(a, stream));
 }
 

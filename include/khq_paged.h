@@ -100,9 +100,10 @@ typedef struct khq_rows {
  * weight) and the half-split rotation of its first rotary_dim dims (pairs
  * i, i + rotary_dim / 2; angle position * theta^(-2 i / rotary_dim)) in one
  * pass over n tokens; with pages, row i's rotated keys and its values go to
- * slot slots[i] (no write for a slot outside the cache).  The many-token form
- * of khq_layer_attention_step's front.  rotary_dim: a multiple of 16, 0 for no
- * rotation.  Outputs overlap no input but their own. */
+ * slot slots[i] (no write for a slot outside the cache; what a slot named twice
+ * holds is not said).  The many-token form of khq_layer_attention_step's front.
+ * rotary_dim: a multiple of 16, 0 for no rotation.  Outputs overlap no input but
+ * their own, and pages whose slots share memory are refused. */
 int khq_qk_norm_rope(const khq_rows* rows, const khq_pages* pages, hipStream_t stream);
 
 /* Queries of one attention call. */
@@ -136,7 +137,9 @@ typedef struct khq_attn_rows {
  * fixed order: results do not change from run to run.  The parts live in ws;
  * with ws NULL in the library's workspace, which khq_workspace_reserve grows
  * before a capture: two graphs that share it must not run at once, and those
- * that may have a ws each (khq_paged_attn_ws_bytes says how large). */
+ * that may have a ws each (khq_paged_attn_ws_bytes says how large).  Calls of
+ * several threads take the library's in turn.
+ * n_tok * H_q is below 2^27, n_seq * H_kv at most 2^21, scale finite. */
 int khq_paged_attn(const khq_attn_rows* rows, const khq_pages* pages, hipStream_t stream);
 
 /* Bytes of workspace that khq_paged_attn uses for these sizes, whatever the

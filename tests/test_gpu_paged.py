@@ -1,6 +1,7 @@
 """The paged cache's operators against plain implementations in 64 bits
 (tests/pagedref.py)."""
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -445,6 +446,43 @@ def test_attn_device_lengths_outside_their_range(device):
     long["table"] = c["table"].clamp(max=3)
     got = run_attn(long)
     assert got.shape == c["q"].shape
+
+
+@pytest.mark.parametrize("n,heads,max_q", [(5, WIDE, 1), (300, WIDE, 300), (700, COMMON, 700)])
+def test_attn_rows_of_many_sequences(n, heads, max_q, device):
+    """cu_q that names the same rows again and again: more row tiles than the batch can have.
+    What the rows hold is not said; the workspace is not left."""
+    c = attn_case([(n, 900)], *heads, 16, F16, 1, device)
+    n_seq, hq, hkv, d = 300, *heads[:3]
+    need = paged.attn_ws_bytes(n, n_seq, hq, hkv, d, max_q)
+    room = torch.full((need + 8192,), 90, dtype=torch.uint8, device=device)
+    wild = dict(c, cu=i32([0, n] * (n_seq // 2) + [0], device), kv=c["kv"].repeat(n_seq),
+                table=c["table"].repeat(n_seq, 1), max_q=max_q)
+    run_attn(wild, workspace=room[4096:4096 + need])
+    assert bool((room[:4096] == 90).all()) and bool((room[4096 + need:] == 90).all())
+
+
+def test_attn_from_two_threads(device):
+    """Threads that launch at once, each on its stream, share the library's workspace."""
+    cases = [attn_case([(1, 6000), (3, 77)], *WIDE, 16, F16, 1, device),
+             attn_case([(90, 3000)], *COMMON, 64, BF16, 5, device)]
+    want = [run_attn(c) for c in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[k].append(run_attn(cases[k]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for outs, w in zip(got, want):
+        assert len(outs) == 20 and all(torch.equal(x, w) for x in outs)
 
 
 def test_attn_workspace_and_streams(device):

@@ -75,6 +75,25 @@ def test_attn_refused(over):
     assert paged.lib().khq_paged_attn(queries(**over), pages(), None) == -100
 
 
+@pytest.mark.parametrize("over", [
+    dict(scale=float("inf")), dict(scale=float("nan")), dict(n_tok=1 << 23, hq=16),
+    dict(n_seq=4096, hq=1024, hkv=1024)])
+def test_attn_sizes_refused(over):
+    over = dict(over)
+    p = pages(hkv=over.pop("hkv", 4), n_pages=1)
+    assert paged.lib().khq_paged_attn(queries(**over), p, None) == -100
+
+
+@pytest.mark.parametrize("over", [dict(page=0), dict(token=0), dict(head=0), dict(head=128)])
+def test_rows_refuse_slots_that_share_memory(over):
+    assert paged.lib().khq_qk_norm_rope(rows(), pages(**over), None) == -100
+
+
+@pytest.mark.parametrize("theta", [float("inf"), -1.0])
+def test_rows_theta_refused(theta):
+    assert paged.lib().khq_qk_norm_rope(rows(theta=theta), pages(), None) == -100
+
+
 def test_attn_workspace_refused():
     need = paged.attn_ws_bytes(4, 2, 24, 4, 256, 4)
     lib = paged.lib()
