@@ -30,20 +30,43 @@ constexpr int PLAN_ONE = 8192;
 // a + b of values up to most <= 2^31, at most most.
 __device__ __forceinline__ uint32_t sat(uint32_t a, uint32_t b, uint32_t most) { return min(a + b, most); }
 
-// Saturating sums of v over the threads before this one; s_w: a word a wavefront.
-__device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t most, uint32_t* s_w) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+// Saturating inclusive sums over the lanes: within rows of 16, then rows to the
+// right of lanes 15, 31 and 47.  (Each step is a register operation; shuffles
+// through LDS and a walk over the wavefronts' sums made three such sums of 512
+// requests 3 us of a plan's 8.)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_from(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t scan_row(uint32_t v, uint32_t most) {
+    v = sat(v, dpp_from<0x111, 0xF>(v), most);  // row_shr 1, 2, 4, 8
+    v = sat(v, dpp_from<0x112, 0xF>(v), most);
+    v = sat(v, dpp_from<0x114, 0xF>(v), most);
+    return sat(v, dpp_from<0x118, 0xF>(v), most);
+}
+__device__ __forceinline__ uint32_t scan(uint32_t v, uint32_t most) {
+    v = scan_row(v, most);
+    v = sat(v, dpp_from<0x142, 0xA>(v), most);  // row_bcast 15, 31
+    return sat(v, dpp_from<0x143, 0xC>(v), most);
+}
+// Saturating sums of v[i] over the threads before this one; s_w: a word a wavefront.
+constexpr int PLAN_WAVES = PLAN_THR / 64;
+static_assert(PLAN_WAVES <= 16, "their sums are a row of lanes");
+template <int N>
+__device__ __forceinline__ void sum_before(uint32_t (&v)[N], uint32_t most, uint32_t (*s_w)[PLAN_WAVES]) {
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t x = __shfl_up(v, o, 64);
-        if (lane >= o) v = sat(v, x, most);
+    for (int i = 0; i < N; i++) {
+        v[i] = scan(v[i], most);
+        if (lane == 63) s_w[i][wv] = v[i];
+        v[i] = dpp_from<0x138, 0xF>(v[i]);  // the lane before's
     }
-    if (lane == 63) s_w[wv] = v;
-    v = __shfl_up(v, 1, 64);
-    v = lane == 0 ? 0 : v;
     __syncthreads();
-    for (int w = 0; w < wv; w++) v = sat(v, s_w[w], most);
-    return v;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t w = scan_row(lane < wv ? s_w[i][lane] : 0u, most);  // (wv is below 16)
+        v[i] = sat(v[i], (uint32_t)__builtin_amdgcn_readlane((int)w, 15), most);
+    }
 }
 
 // First index in [0, n) whose s[i + 1] > x, s increasing (the last if none; s[n] is not read).
@@ -73,7 +96,7 @@ struct Sums {
     int head, count;
 };
 struct PlanLds {
-    uint32_t w[3][PLAN_THR / 64];
+    uint32_t w[3][PLAN_WAVES];
     int taken, refused, n_back;  // of all requests, after the next barrier
 };
 
@@ -81,7 +104,8 @@ __device__ __forceinline__ void plan_sums(const PlanArgs& a, int per, Sums& s, P
     const uint32_t most_q = (uint32_t)a.n_tok + 1, most_p = (uint32_t)a.n_pages + 1;
     const int head = a.state[0], count = a.state[1];
     if (threadIdx.x == 0) lds.taken = lds.refused = lds.n_back = 0;
-    uint32_t rows = 0;
+    uint32_t of_rows[1] = {0};
+    uint32_t& rows = of_rows[0];
 #pragma unroll
     for (int i = 0; i < PLAN_SEQS; i++) {
         const int sq = threadIdx.x * per + i;
@@ -94,7 +118,7 @@ __device__ __forceinline__ void plan_sums(const PlanArgs& a, int per, Sums& s, P
     s.head = head % a.n_pages;
     s.head += s.head < 0 ? a.n_pages : 0;
     s.count = min(max(count, 0), a.n_pages);
-    rows = sum_before(rows, most_q, lds.w[0]);
+    sum_before(of_rows, most_q, lds.w);
     uint32_t need = 0, back = 0, mine[PLAN_SEQS];
 #pragma unroll
     for (int i = 0; i < PLAN_SEQS; i++) {
@@ -108,7 +132,9 @@ __device__ __forceinline__ void plan_sums(const PlanArgs& a, int per, Sums& s, P
         need = sat(need, min(mine[i], most_p), most_p);
         back = sat(back, s.q[i] < 0 ? min((uint32_t)min(s.has[i], a.table_ld), most_p) : 0, most_p);
     }
-    const uint32_t need0 = sum_before(need, most_p, lds.w[1]), back0 = sum_before(back, most_p, lds.w[2]);
+    uint32_t before[2] = {need, back};
+    sum_before(before, most_p, lds.w + 1);
+    const uint32_t need0 = before[0], back0 = before[1];
     int taken = 0, refused = 0;
 #pragma unroll
     for (int i = 0; i < PLAN_SEQS; i++) {
