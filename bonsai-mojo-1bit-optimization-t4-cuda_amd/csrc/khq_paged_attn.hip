@@ -1140,18 +1140,24 @@ __global__ __launch_bounds__(64 * JW) void attn_join_kernel(AttnArgs a, Part pl,
 
 // What a call of these sizes launches.
 struct Plan {
-    bool tile;  // sequences of many rows there may be
+    bool tile;  // tiles for sequences of many rows
     Part pl, ps;
     int blocks, waves, kg, joins, join_waves, row_step;
 };
 size_t part_floats(const Part& pt, int d) { return (size_t)2 * pt.slots * pt.rows * (d + 2); }
 
-// max_q only chooses between the two launches: either serves every sequence.
-Plan plan_of(int n_tok, int n_seq, int H_q, int H_kv, int d, int max_q) {
+// The sizes only choose between the two launches: either serves every sequence.
+// Rows a sequence may have up to max_q go by 16 where there are no more, or
+// where few keys (max_kv: what the table holds) make little work of them: a tile
+// starts and ends in some 20 us, however few its keys.  A prompt of 128, 24 heads
+// of 256: 14.5 us by 16, 23.4 in tiles; of 256: 18.4 and 29.9; 128 tokens after
+// 1,024, past the bound: 38.3 and 34.5; 16 after 8,192, at it: 38.7 and 39.0.
+constexpr double LIGHT = 3.0 * (1 << 28);
+Plan plan_of(int n_tok, int n_seq, int H_q, int H_kv, int d, int max_q, double max_kv) {
     const int n_rep = H_q / H_kv, seqs = std::min(n_tok, n_seq);
     const long long rows = (long long)n_tok * n_rep;
     Plan p{};
-    p.tile = (long long)max_q * n_rep > SMALL_ROWS;
+    p.tile = (long long)max_q * n_rep > SMALL_ROWS && (double)n_tok * H_q * d * max_kv > LIGHT;
     if (p.tile) {
         // 256 dims fill LDS with one block's keys and values: 8 wavefronts on 256
         // rows or, where those tiles would be fewer than the CUs, 128.  Else two
@@ -1187,7 +1193,8 @@ constexpr int stream_bytes(int waves, int d) { return waves * 16 * (d + 6) * (in
 
 template <typename T, int D>
 hipError_t launch(const AttnArgs& a, hipStream_t st) {
-    const Plan p = plan_of(a.r.n_tok, a.r.n_seq, a.r.H_q, a.p.H_kv, D, a.r.max_q);
+    const Plan p = plan_of(a.r.n_tok, a.r.n_seq, a.r.H_q, a.p.H_kv, D, a.r.max_q,
+                           (double)a.r.table_ld * a.p.page_size);
     if (p.tile) {
         constexpr int NW = D == 256 ? 8 : 4;
         constexpr int bytes = 4 * 64 * 2 * D + TAB * (int)sizeof(long long) + (D == 256 ? 8 * 2 * 1024 : 0);
@@ -1210,7 +1217,8 @@ hipError_t launch(const AttnArgs& a, hipStream_t st) {
 }  // namespace
 
 size_t attn_ws_bytes(int n_tok, int n_seq, int H_q, int H_kv, int head_dim, int max_q) {
-    const Plan p = plan_of(n_tok, n_seq, H_q, H_kv, head_dim, max_q);
+    // (tiles' partial results are more than those by 16 rows)
+    const Plan p = plan_of(n_tok, n_seq, H_q, H_kv, head_dim, max_q, 1e10);
     return (part_floats(p.pl, head_dim) + part_floats(p.ps, head_dim)) * sizeof(float);
 }
 

@@ -265,6 +265,19 @@ def test_rows_edges(device):
 
 
 # ---------------------------------------------------------------------- attn
+@pytest.fixture(params=["tight", "wide"])
+def table_width(request, monkeypatch):
+    """Tables that hold just the longest sequence, and tables of 2^22 tokens: what they could
+    hold decides how many rows are taken at once."""
+    if request.param == "wide":
+        def wide_case(*args, case=attn_case, **kw):
+            c = case(*args, **kw)
+            more = (1 << 22) // c["kp"].shape[1] - c["table"].shape[1]
+            return dict(c, table=torch.nn.functional.pad(c["table"], (0, more), value=-1))
+
+        monkeypatch.setitem(globals(), "attn_case", wide_case)
+
+
 def attn_case(lens, hq, hkv, d, page, dtype, seed, device, gate=False, fill=None, pad=0):
     q_len, kv = [a for a, _ in lens], [b for _, b in lens]
     kp, vp, table = pagedref.rand_cache(len(lens), kv, page, hkv, d, dtype, seed, device, fill=fill)
@@ -320,6 +333,7 @@ CHUNKS = [(5, 5), (1, 90), (37, 200), (0, 40), (64, 64), (3, 3), (130, 131), (2,
     ((3, 3, 256), 1, F16, CHUNKS, False), (WIDE, 64, F16, [(1, 1)], True),
     (WIDE, 16, BF16, [(1, 4500)], False), ((16, 1, 256), 64, F16, [(2, 1025), (4, 90)], True),
     (COMMON, 64, F16, [(256, 1300)], False), (WIDE, 32, F16, [(300, 300)], False)])
+@pytest.mark.usefixtures("table_width")
 def test_attn(heads, page, dtype, lens, gate, device):
     say("attn", heads, page, dtype, lens, gate)
     c = attn_case(lens, *heads, page, dtype, 11, device, gate=gate, fill=math.nan, pad=3)
@@ -330,6 +344,7 @@ def test_attn(heads, page, dtype, lens, gate, device):
 
 
 @pytest.mark.parametrize("heads,dtype", [(WIDE, F16), (COMMON, BF16), (SMALL, F16)])
+@pytest.mark.usefixtures("table_width")
 def test_attn_rows_that_see_nothing(heads, dtype, device):
     """More rows than tokens, no tokens at all, lengths below zero."""
     lens = [(6, 2), (4, 0), (40, 33), (1, 0), (1, 5), (300, 20)]
@@ -344,6 +359,7 @@ def test_attn_rows_that_see_nothing(heads, dtype, device):
 @pytest.mark.parametrize("heads,dtype,lens", [
     (WIDE, F16, [(5, 60), (2, 2)]), (WIDE, F16, [(70, 100)]), (COMMON, BF16, [(3, 40), (4, 4)]),
     (COMMON, F16, [(90, 90), (1, 50)]), (SMALL, BF16, [(9, 77)]), ((2, 2, 64), F16, [(200, 233)])])
+@pytest.mark.usefixtures("table_width")
 def test_attn_nonfinite_in_masked_places(heads, dtype, lens, device):
     """A new token's infinities and NaN reach the rows that see it, and no other."""
     c = attn_case(lens, *heads, 16, dtype, 21, device)
@@ -367,6 +383,7 @@ def test_attn_nonfinite_in_masked_places(heads, dtype, lens, device):
     check_attn(c, run_attn(c), (want, bound))
 
 
+@pytest.mark.usefixtures("table_width")
 def test_attn_large_scores_and_lowest_values(device):
     """Scores far apart, keys of the type's largest values, a mask's lowest value as key."""
     for heads, lens in ((WIDE, [(1, 300), (4, 50)]), (COMMON, [(90, 200)])):
@@ -388,6 +405,7 @@ def test_attn_large_scores_and_lowest_values(device):
     check_attn(c, out)
 
 
+@pytest.mark.usefixtures("table_width")
 def test_attn_strides_and_alignment(device):
     """Pages as [pages][heads][tokens][dims] of one tensor, queries at odd addresses and
     strides, heads before tokens, an output of other strides."""
@@ -410,6 +428,7 @@ def test_attn_strides_and_alignment(device):
         assert torch.equal(got, want)
 
 
+@pytest.mark.usefixtures("table_width")
 def test_attn_max_q_is_only_a_hint(device):
     for heads, lens in ((WIDE, CHUNKS), (COMMON, CHUNKS)):
         c = attn_case(lens, *heads, 64, F16, 9, device)
@@ -418,6 +437,7 @@ def test_attn_max_q_is_only_a_hint(device):
             check_attn(c, run_attn(c, max_q=m), ref)
 
 
+@pytest.mark.usefixtures("table_width")
 def test_attn_bad_pages(device):
     """An entry outside the cache makes its sequence's rows that see it NaN, and no others."""
     for heads, lens in ((WIDE, [(1, 200), (1, 300), (1, 40)]), (COMMON, [(50, 200), (60, 300), (1, 40)])):
@@ -431,6 +451,7 @@ def test_attn_bad_pages(device):
             assert bool(got[a:b].isnan().all())
 
 
+@pytest.mark.usefixtures("table_width")
 def test_attn_device_lengths_outside_their_range(device):
     """cu_q past the batch or going back, lengths past the table: nothing outside is touched,
     the sequences that are in order are right."""
@@ -449,6 +470,7 @@ def test_attn_device_lengths_outside_their_range(device):
 
 
 @pytest.mark.parametrize("n,heads,max_q", [(5, WIDE, 1), (300, WIDE, 300), (700, COMMON, 700)])
+@pytest.mark.usefixtures("table_width")
 def test_attn_rows_of_many_sequences(n, heads, max_q, device):
     """cu_q that names the same rows again and again: more row tiles than the batch can have.
     What the rows hold is not said; the workspace is not left."""
@@ -462,6 +484,7 @@ def test_attn_rows_of_many_sequences(n, heads, max_q, device):
     assert bool((room[:4096] == 90).all()) and bool((room[4096 + need:] == 90).all())
 
 
+@pytest.mark.usefixtures("table_width")
 def test_attn_from_two_threads(device):
     """Threads that launch at once, each on its stream, share the library's workspace."""
     cases = [attn_case([(1, 6000), (3, 77)], *WIDE, 16, F16, 1, device),
@@ -485,6 +508,7 @@ def test_attn_from_two_threads(device):
         assert len(outs) == 20 and all(torch.equal(x, w) for x in outs)
 
 
+@pytest.mark.usefixtures("table_width")
 def test_attn_workspace_and_streams(device):
     """A caller's workspace, and calls on several streams at once, each with its own."""
     cases = [attn_case([(1, 900), (1, 400), (3, 77)], *WIDE, 16, F16, s, device) for s in range(3)]
