@@ -230,6 +230,20 @@ __device__ __forceinline__ Schedule schedule(const AttnArgs& a, const Part& pt, 
     }
     return sc;
 }
+// Row tile, from the last, that is started q-th of a lone sequence's.  Longest
+// first, each round of blocks (w tiles of every head) ends the rounds before it
+// evenly: a block that took the longest gets the shortest.  So an even number of
+// rounds ends as one; of an odd number the last one starts as one and ends
+// unevenly (a prompt of 8,192, 24 heads of 256, is 3: a tenth of the chip idle).
+// There the round before it takes every other tile first, then the others: the
+// blocks then come free spread as the last round's tiles are long.
+__device__ __forceinline__ int started(const AttnArgs& a, const Part& pt, int q, int tiles) {
+    const int w = a.by_kv.div(pt.slots);
+    if (tiles <= 2 * w || w < 2) return q;
+    const int rounds = (int)((uint32_t)(tiles + w - 1) / (uint32_t)w), i = q - (rounds - 2) * w, half = (w + 1) >> 1;
+    if (rounds % 2 == 0 || i < 0 || i >= w) return q;
+    return q - i + (i < half ? 2 * i : 2 * (i - half) + 1);
+}
 // Item x, below sc.total.
 __device__ __forceinline__ Item item_of(const AttnArgs& a, const Part& pt, const Schedule& sc, int x,
                                         bool joining) {
@@ -261,7 +275,8 @@ __device__ __forceinline__ Item item_of(const AttnArgs& a, const Part& pt, const
     it.head = j - k * h_kv;
     const int q = joining || it.n_split == 1 ? k : (int)((uint32_t)k / (uint32_t)it.n_split);
     it.split = joining ? 0 : k - q * it.n_split;
-    it.qt = tiles - 1 - q;  // row tiles from the last
+    const bool lone = a.r.n_seq == 1 && it.n_split == 1;
+    it.qt = tiles - 1 - (lone ? started(a, pt, q, tiles) : q);  // row tiles from the last
     it.part = from(part) + q * it.n_split * h_kv + it.head;
     return it;
 }

@@ -428,6 +428,17 @@ def test_attn_strides_and_alignment(device):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("n,heads", [(900, 128), (1100, 128), (1536, 128), (1100, 256)])
+def test_attn_rounds_of_blocks(n, heads, device):
+    """A lone prompt of two, three, three full and five rounds of blocks (tiles of 128 rows,
+    512 at once): every row tile is some block's.  Checked for four of the heads."""
+    c = attn_case([(n, n)], heads, heads, 64, 64, F16, 12, device)
+    out = run_attn(c)
+    some = [0, 1, 77, heads - 1]
+    few = dict(c, q=c["q"][:, some], kp=c["kp"][:, :, some], vp=c["vp"][:, :, some])
+    check_attn(few, out[:, some])
+
+
 @pytest.mark.usefixtures("table_width")
 def test_attn_max_q_is_only_a_hint(device):
     for heads, lens in ((WIDE, CHUNKS), (COMMON, CHUNKS)):
