@@ -9,10 +9,10 @@
 // (schedule below), which for one sequence is a few scalar operations and for
 // some hundred one pass of a wavefront, about a microsecond.
 //
-// Two kernels share the sequences by their row count: up to 16 rows (a decode
-// step's 6 of 24 / 4 heads) stream keys and values through registers
-// (stream_item), more go in tiles of 128 or 256 rows that share keys
-// and values in LDS (tile_item).
+// Row tiles come in two sizes: up to 16 rows of a sequence (a decode step's 6 of
+// 24 / 4 heads), and all rows of a light batch, stream keys and values through
+// registers (stream_item); more go in tiles of 128 or 256 rows that share keys
+// and values in LDS (tile_item).  One launch serves both, or the first alone.
 #include "khq_mfma_util.h"
 #include "khq_paged_internal.h"
 
@@ -333,7 +333,12 @@ __device__ __forceinline__ long long uniform(long long x) {
 // product's K index 8 g + j stands for key 4 g + j (j < 4) and 16 + 4 g + j - 4;
 // a lane loads those 8 keys' values of 8 consecutive dims and transposes them
 // in its registers (32 byte permutes), dim 8 m + t standing for row m of
-// product t.  No LDS and no barrier until the block's wavefronts join.
+// product t.  No LDS and no barrier until the block's wavefronts join.  Bound:
+// memory; what it takes is loads under way, so a tile's 32 of 16 bytes are all
+// issued before the first product, 256 registers a lane and two blocks of 4 a
+// CU.  24 / 4 heads of 256 in fp16: 32 sequences of 1K to 16K tokens, 680 MB in
+// 130 us (5.2 TB/s; a copy of 2 GB runs at 4.9), one of 131,071, 537 MB in 98
+// (5.5); 512 tokens, of which latency is all, 8.6.
 template <typename T, int D, int NW>
 __device__ __forceinline__ void stream_item(const AttnArgs& a, const Part& pt, const Item& it, char* smem) {
     constexpr int KS = D / 32;                             // K steps of a score
@@ -695,14 +700,20 @@ __device__ __forceinline__ void store_row4(const AttnArgs& a, const Item& it, in
 
 // 32 rows a wavefront on 32x32x16 MFMAs, 64 keys and values at a time in one of
 // two LDS slots while the next ones are on their way into the other, straight
-// from memory.  KG 1: eight wavefronts of 256 rows, each taking all 64 keys; KG
-// 2: 128 rows, each wavefront 32 of the 64 keys of its rows, the two halves
+// from memory.  KG 1: NW wavefronts of 32 NW rows, each taking all 64 keys; KG 2:
+// 128 rows, each wavefront 32 of the 64 keys of its rows, the two halves
 // joined at the end.  S^T = K Q^T: its result (row = lane % 32, key 8 (e / 4) +
 // 4 (lane / 32) + e % 4 in register e) is the B operand of O^T += V^T P^T when
 // that product's K index i of step s stands for key 16 s + 8 (i / 4) + 4 (lane /
 // 32) + i % 4, which is how V is read, transposed on its way out of LDS.
 // 16-byte pieces of a row are permuted (K: piece ^ key, V: piece ^ 4 key) so
-// that the lanes of a read meet all banks.
+// that the lanes of a read meet all banks (no conflict counted).  Bound: the
+// matrix cores, beside which a unit's 64 products a wavefront put some 320 vector
+// instructions (maximum, exponentials, packing, addresses) and 130 LDS reads:
+// busy half of the cycles, at the 2.0 GHz that the power leaves.  A prompt of
+// 8,192, 24 / 4 heads of 256 in fp16: 824 us, 1,001 TFLOP/s (large library
+// products: 1,228 to 1,304); 128 tokens after 32,768, KG 2: 803 TFLOP/s; 32 / 8
+// heads of 128, two blocks of 4 wavefronts a CU, a prompt of 8,192: 594 us, 926.
 template <typename T, int D, int KG, int NW>
 __device__ __forceinline__ void tile_item(const AttnArgs& a, const Part& pt, const Item& it, char* lds) {
     constexpr int NS = D / 16, ND = D / 32;  // K steps of a score, dim tiles
@@ -743,13 +754,13 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Part& pt, con
             if (bad) s_bad = 1;
         }
     };
-    // A unit into a slot: 8 keys a wavefront, NL loads of 1 KB of K and of V.  A
+    // A unit into a slot: WK keys a wavefront, NL loads of 1 KB of K and of V.  A
     // load takes the address unit 16 cycles, and a wavefront waits where others'
-    // are before its own.  So the two wavefronts of a SIMD, i and i + 4, take
-    // turns: i + 4 loads while i has the matrix cores for its scores, and i
-    // loads while i + 4 has them (all eight at once, or between their products,
-    // left the matrix cores idle half the time: 890 us of 8,192 tokens, not 8).
-    // Where the 8 keys lie in one page, as they do in pages of a multiple of 8,
+    // are before its own.  So of 8 wavefronts the two of a SIMD, i and i + 4, take
+    // turns: i + 4 loads while i has the matrix cores for its scores, and i loads
+    // while i + 4 has them (all eight at once, or between their products, left the
+    // matrix cores idle half the time: 890 us of a prompt of 8,192 for 840).
+    // Where the WK keys lie in one page, as they do in pages of a multiple of WK,
     // an address is a scalar and a lane's constant; else each lane looks its
     // key up.
     const char* const kh = (const char*)a.p.k + 2 * (it.head * a.p.head_stride);
@@ -1122,8 +1133,8 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, 2) void attn_stream_kernel(AttnA
 }
 
 // Tiles of the sequences of many rows, then those of few: a continuous batch's
-// decoding sequences run beside its chunks (two launches one after the other
-// and two joins took 105 us of a batch of 24).
+// decoding sequences run beside its chunks (24 sequences in bf16, 32 / 8 heads of
+// 128: 78 us; two launches one after the other and two joins took 105).
 template <typename T, int D, int KG, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_tile_kernel(AttnArgs a, Part pl, Part ps) {
     const Schedule sl = schedule<true>(a, pl, false);
@@ -1136,6 +1147,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_tile_kernel(AttnArgs a, Part 
     if (x < sc.total) stream_item<T, D, NW>(a, ps, item_of(a, ps, sc, x, false), dyn_lds);
 }
 
+// The splits' partial results, in order.  Bound: latency where they are few (4 us
+// of one token after 511, 6 after 131,071), else their bytes, which the launch
+// before has to have written back (128 rows after 8,192: 31 MB, 10 us).
 // row_step: rows of a row tile of 16 that there should be (others follow).
 template <typename T, int D, int JW>
 __global__ __launch_bounds__(64 * JW) void attn_join_kernel(AttnArgs a, Part pl, Part ps, int row_step) {
@@ -1196,7 +1210,9 @@ Plan plan_of(int n_tok, int n_seq, int H_q, int H_kv, int d, int max_q, double m
     p.blocks = (int)(large + p.pl.slots + small + p.ps.slots);
     p.row_step = (int)std::min<long long>(16, (long long)max_q * n_rep);
     const long long items = std::min<long long>(p.ps.slots, small) * p.row_step;
-    // few rows may have many splits
+    // Few rows may have many splits (one token after 131,071: 105 us with 16
+    // wavefronts a row, 110 with 4); many rows fill the chip with 4 (32 sequences: a
+    // join of 6 us, with 8 wavefronts 11).
     p.join_waves = !p.tile && items <= 64 ? 16 : 4;
     const long long pieces = std::min<long long>(p.pl.slots, large) * (p.pl.rows / 32) * (d / 8);
     p.joins = (int)std::min<long long>(items + (pieces + p.join_waves - 1) / p.join_waves, 2048);

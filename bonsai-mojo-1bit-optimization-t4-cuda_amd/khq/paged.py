@@ -225,7 +225,8 @@ def qk_norm_rope(q, k, q_out, *, positions=None, pos0: int = 0, q_weight=None, k
     if dt not in _DTYPES:
         raise TypeError(f"q, k: dtype {dt}, expected float16 or bfloat16")
     if first.dim() != 3 or first.shape[2] not in _HEAD_DIMS:
-        raise ValueError(f"q, k: shape {tuple(first.shape)}, expected [tokens][heads][64, 128 or 256]")
+        raise ValueError(f"q, k: shape {tuple(first.shape)}, expected "
+                         "[tokens][heads][64, 128 or 256]")
     n, _, d = first.shape
     none = (0, 0, 0)
     q_at = q_out_at = k_at = k_out_at = k_normed_at = v_at = none
