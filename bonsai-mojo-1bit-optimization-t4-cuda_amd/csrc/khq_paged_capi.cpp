@@ -67,6 +67,7 @@ int khq_qk_norm_rope(const khq_rows* rows, const khq_pages* pages, hipStream_t s
                   (pages->H_kv > 1 && pages->head_stride < r.head_dim)))
         return -100;  // slots that share memory, as an expanded tensor's do
     if (!pages && r.k && !r.k_out && !r.k_normed) return -100;  // nothing to leave the keys in
+    if (!r.positions && r.pos0 > 0x7fffffff - r.n) return -100;  // the last position
     if (r.n == 0) return 0;
     khq::paged::RowsArgs a{};
     a.r = r;

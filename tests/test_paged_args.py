@@ -113,6 +113,10 @@ def test_rows_refused(over):
     assert paged.lib().khq_qk_norm_rope(rows(**over), pages(), None) == -100
 
 
+def test_rows_positions_past_32_bits_refused():
+    assert paged.lib().khq_qk_norm_rope(rows(pos=0, n=4, pos0=0x7fffffff - 3), pages(), None) == -100
+
+
 def test_rows_need_somewhere_to_go():
     assert paged.lib().khq_qk_norm_rope(rows(), None, None) == -100
     assert paged.lib().khq_qk_norm_rope(rows(hkv=8), pages(), None) == -100
