@@ -850,14 +850,21 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Part& pt, con
             const char* const kb = ks + at;
             const char* const vb = vs + at;
             const int ka = opaque(k_at), va = opaque(v_at);  // (the permuted places: a xor each)
-            // An operand's read is AHEAD products before its own.
+            // An operand's read is AHEAD products before its own.  (256 dims: the
+            // permutation leaves a place's 256s alone, so two reads share a xor.)
+            auto step = [](int n) { return D == 256 ? (n >> 1) + (n & 1) * 8 : n; };
+            auto tile = [](int n) { return D == 256 ? (n >> 1) + (n & 1) * 4 : n; };
             x8 kf[AHEAD + 1];
-            auto read_k = [&](int st) {
-                kf[st % (AHEAD + 1)] = *reinterpret_cast<const x8*>(kb + (ka ^ (st << 5)));
+            auto read_k = [&](int n) {
+                const int st = step(n);
+                kf[n % (AHEAD + 1)] = *reinterpret_cast<const x8*>(
+                    D == 256 ? kb + (ka ^ ((st & 7) << 5)) + (st >> 3) * 256 : kb + (ka ^ (st << 5)));
             };
-            u4 vf[AHEAD + 1];  // dim tile n / 2, K step n % 2
+            u4 vf[AHEAD + 1];  // dim tile(n / 2), K step n % 2
             auto read_v = [&](int n) {
-                const char* const p = vb + (va ^ ((n >> 1) << 6)) + 16 * (n & 1) * ROW;
+                const int i = tile(n >> 1);
+                const char* const p = (D == 256 ? vb + (va ^ ((i & 3) << 6)) + (i >> 2) * 256 : vb + (va ^ (i << 6))) +
+                                      16 * (n & 1) * ROW;
                 const u2 lo = read_tr(p), hi = read_tr(p + 8 * ROW);
                 vf[n % (AHEAD + 1)] = u4{lo.x, lo.y, hi.x, hi.y};
             };
@@ -865,13 +872,14 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Part& pt, con
 #pragma unroll
             for (int e = 0; e < 16; e++) sc[e] = 0.0f;
 #pragma unroll
-            for (int st = 0; st < AHEAD; st++) read_k(st);
+            for (int n = 0; n < AHEAD; n++) read_k(n);
 #pragma unroll
-            for (int st = 0; st < NS; st++) {
-                if (st + AHEAD < NS) read_k(st + AHEAD);
-                else read_v(st + AHEAD - NS);
+            for (int n = 0; n < NS; n++) {
+                const int st = step(n);
+                if (n + AHEAD < NS) read_k(n + AHEAD);
+                else read_v(n + AHEAD - NS);
                 __builtin_amdgcn_sched_barrier(0);
-                sc = mfma32(kf[st % (AHEAD + 1)],
+                sc = mfma32(kf[n % (AHEAD + 1)],
                             st < QL ? *reinterpret_cast<const x8*>(lds + q_at + st * 1024) : qb[max(st - QL, 0)], sc);
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -951,7 +959,8 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Part& pt, con
                 u4 v = vf[n % (AHEAD + 1)];
                 if constexpr (MASKED)  // ... and leave the product
                     v = u4{finite_pair<T>(v.x), finite_pair<T>(v.y), finite_pair<T>(v.z), finite_pair<T>(v.w)};
-                acc[n >> 1] = mfma32(__builtin_bit_cast(x8, v), pb[n & 1], acc[n >> 1]);
+                const int i = tile(n >> 1);
+                acc[i] = mfma32(__builtin_bit_cast(x8, v), pb[n & 1], acc[i]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
