@@ -711,8 +711,8 @@ __device__ __forceinline__ void store_row4(const AttnArgs& a, const Item& it, in
 // matrix cores, beside which a unit's 64 products a wavefront put some 320 vector
 // instructions (maximum, exponentials, packing, addresses) and 130 LDS reads:
 // busy half of the cycles, at the 2.0 GHz that the power leaves.  A prompt of
-// 8,192, 24 / 4 heads of 256 in fp16: 824 us, 1,001 TFLOP/s (large library
-// products: 1,228 to 1,304); 128 tokens after 32,768, KG 2: 803 TFLOP/s; 32 / 8
+// 8,192, 24 / 4 heads of 256 in fp16: 791 to 809 us, 1,020 to 1,043 TFLOP/s (large
+// library products: 1,228 to 1,304); 128 tokens after 32,768, KG 2: 803; 32 / 8
 // heads of 128, two blocks of 4 wavefronts a CU, a prompt of 8,192: 594 us, 926.
 template <typename T, int D, int KG, int NW>
 __device__ __forceinline__ void tile_item(const AttnArgs& a, const Part& pt, const Item& it, char* lds) {
